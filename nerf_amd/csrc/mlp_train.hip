@@ -71,6 +71,12 @@ __host__ __device__ inline float auto_gscale(unsigned absmax_bits, int target_ex
 #endif
 }
 
+// Clears the status block.  A kernel and not hipMemsetAsync: a backward pass may be captured into a
+// graph, and memset nodes do not replay reliably.
+__global__ __launch_bounds__(kStatusBytes / 4) void clear_status_kernel(unsigned* __restrict__ status) {
+    status[threadIdx.x] = 0u;
+}
+
 __global__ __launch_bounds__(256) void draw_absmax_kernel(const float4* __restrict__ d_raw, int64_t n,
                                                           unsigned* __restrict__ status) {
     __shared__ unsigned part[4];
@@ -1107,8 +1113,8 @@ NERF_API int nerf_mlp_backward(const void* packed_bwd, const void* act, const fl
     if (cus <= 0) return NERF_FAIL(NERF_E_UNSUPPORTED, "nerf_mlp_backward: no current device");
 
     unsigned* status = (unsigned*)partial;
-    hipError_t e = hipMemsetAsync(status, 0, kStatusBytes, st);
-    if (e != hipSuccess) return NERF_FAIL((int)e, "nerf_mlp_backward(memset): %s", hipGetErrorString(e));
+    clear_status_kernel<<<1, kStatusBytes / 4, 0, st>>>(status);
+    if (int rc = check_launch("nerf_mlp_backward(clear)")) return rc;
     {
         const int64_t want = (n_points + 255) / 256;
         draw_absmax_kernel<<<(unsigned)(want < 512 ? want : 512), 256, 0, st>>>((const float4*)d_raw, n_points, status);
