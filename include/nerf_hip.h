@@ -35,6 +35,11 @@ extern "C" {
 #define NERF_E_ARG (-1)        /* null pointer / non-positive size / unsupported width      */
 #define NERF_E_UNSUPPORTED (-2) /* shape outside what the kernels are built for              */
 
+/* element types of the 8-bit dense-layer entry points */
+#define NERF_F32 0
+#define NERF_F16 1
+#define NERF_BF16 2
+
 typedef void* nerf_stream_t;
 
 int nerf_abi_version(void);
@@ -285,6 +290,51 @@ int nerf_photometric_loss(const float* rgb, const float* rgb0, const float* targ
  * writes NaN gradients when its fp16 chain saturated, and such a step must not reach the weights. */
 int nerf_adam_step(float* theta, const float* g, float* m, float* v, int64_t n, float lr_t,
                    float beta1, float beta2, float eps, nerf_stream_t stream);
+
+/* ---- dense layers in 8 bits ----------------------------------------------------------------- */
+
+/* One dense layer y = relu(x W + b) (run_nerf_helpers.py:83-112) of a network that is queried or trained
+ * layer by layer, for any widths from 1 to 65536.  Neither 8-bit format has a counterpart in the reference.
+ * Types: NERF_F32, NERF_F16, NERF_BF16.  ld*: distance of two rows in elements.
+ *
+ * Rows in 8 bits: q [n][kp], kp = k rounded up to 64, zeros behind column k; scale [n].  An element is
+ * q * scale.  scale = max|x| / 127 of the row (0, and zeros, below 2^-100), or with pow2 the smallest
+ * power of two at or above that, at least 2^-126; q = x / scale rounded, halves to even.  A row that
+ * holds an infinity or NaN gets the scale NaN and zeros.
+ * mask: [n][kp / 8] bytes or NULL; bit f & 7 of byte f >> 3 = (x[f] > 0): what the gradient of a ReLU
+ * whose output x is needs.  q must be 16-byte aligned. */
+int nerf_quantize_rows(const void* x, int dtype, int64_t n, int k, int64_t ldx, int pow2, signed char* q,
+                       float* scale, unsigned char* mask, nerf_stream_t stream);
+
+/* W [k][m] fp32 (Keras kernel [in, out]) -> integers and one scale per output channel (formed as for
+ * rows), laid out for the matrix unit; with pow2 also the transposed copy the input gradient reads.
+ * packed: nerf_int8_packed_bytes(k, m, pow2) bytes (0: widths out of range), 16-byte aligned. */
+size_t nerf_int8_packed_bytes(int k, int m, int pow2);
+int nerf_int8_pack(const float* w, int k, int m, int pow2, void* packed, nerf_stream_t stream);
+
+/* y [n][m] = ((sum_f q[i][f] p[f][j]) * channel scale j) * row scale i (+ bias[j]) (+ addend[i][j]), then
+ * relu when asked; the integer sums are exact, every later step is rounded to fp32, the result to y's
+ * type.  bias [m] or NULL; addend: [n][m] of any of the three types or NULL; y must not overlap an
+ * input. */
+int nerf_linear_int8(const signed char* q, const float* scale, int64_t n, int k, const void* packed, int m,
+                     const float* bias, const void* addend, int addend_dtype, int64_t ldadd, int relu,
+                     void* y, int dtype, int64_t ldy, nerf_stream_t stream);
+
+/* dx [n][k] = dz [n][m] times the transposed weights as the forward pass used them (packed with pow2 only:
+ * they are then exact in bf16), zero where the bit of `mask` is 0.  dz is taken as the exact sum of 1, 2
+ * or 3 bf16 terms (bf16, fp16, fp32): every product is exact, sums are fp32.  dx has dz's type. */
+int nerf_linear_int8_grad_input(const void* dz, int dtype, int64_t n, int m, int64_t lddz, const void* packed, int k,
+                                const unsigned char* mask, void* dx, int64_t lddx, nerf_stream_t stream);
+
+/* dw [k][m] = sum_i q[i][f] scale[i] dz[i][j] and db [m] = sum_i dz[i][j], fp32, from the rows a forward pass
+ * kept.  The scales must be powers of two (rows made with pow2): the products are then exact; another
+ * scale times dz would be rounded to the bf16 terms of dz's type.  n >= 1.
+ * workspace: nerf_linear_int8_grad_weight_bytes(n, k, m) bytes (may be 0).  The same inputs give the same
+ * bits. */
+size_t nerf_linear_int8_grad_weight_bytes(int64_t n, int k, int m);
+int nerf_linear_int8_grad_weight(const signed char* q, const float* scale, int64_t n, int k, const void* dz,
+                                 int dtype, int m, int64_t lddz, float* dw, float* db, void* workspace,
+                                 size_t workspace_bytes, nerf_stream_t stream);
 
 #ifdef __cplusplus
 }

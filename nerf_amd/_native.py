@@ -50,6 +50,13 @@ SIGNATURES = {
     "nerf_mse_loss_fwd_bwd": (_I, [_P, _P, _L, _F, _F, _P, _P, _P]),
     "nerf_photometric_loss": (_I, [_P, _P, _P, _L, _F, _P, _P, _P, _P]),
     "nerf_adam_step": (_I, [_P, _P, _P, _P, _L, _F, _F, _F, _F, _P]),
+    "nerf_quantize_rows": (_I, [_P, _I, _L, _I, _L, _I, _P, _P, _P, _P]),
+    "nerf_int8_packed_bytes": (_c.c_size_t, [_I, _I, _I]),
+    "nerf_int8_pack": (_I, [_P, _I, _I, _I, _P, _P]),
+    "nerf_linear_int8": (_I, [_P, _P, _L, _I, _P, _I, _P, _P, _I, _L, _I, _P, _I, _L, _P]),
+    "nerf_linear_int8_grad_input": (_I, [_P, _I, _L, _I, _L, _P, _I, _P, _P, _L, _P]),
+    "nerf_linear_int8_grad_weight_bytes": (_c.c_size_t, [_L, _I, _I]),
+    "nerf_linear_int8_grad_weight": (_I, [_P, _P, _L, _I, _P, _I, _I, _L, _P, _P, _P, _c.c_size_t, _P]),
 }
 
 _lib = None

@@ -1,0 +1,142 @@
+// Pieces shared by the 8-bit dense-layer kernels (int8_quantize.hip, int8_linear.hip,
+// int8_grad_weight.hip): number formats, the layout of packed weights, loads and stores of rows of any type
+// and alignment.
+//
+// Rows: q [n][kp] int8, kp = k rounded up to 64, zeros behind column k; one fp32 scale per row;
+// optionally one bit per element (element > 0), bit f & 7 of byte f >> 3 of a row of kp / 8 bytes.
+//
+// Packed weights of W [k][m] (Keras [in, out]), mp = m rounded up to 64:
+//   float scale[mp]                            one per output channel, 0 behind m
+//   int8 fragments [mp/64][kp/64][4][64][16]   the integers, A operands of v_mfma_i32_16x16x64_i8
+//   bf16 fragments [kp/64][mp/32][4][64][8]    only with power-of-two scales: integer x scale (exact in
+//                                              bf16: 7 bits), A operands of v_mfma_f32_16x16x32_bf16
+// A fragment is 1 KiB: lane = row (16 output features) + 16 x piece of the contraction (16 integers or
+// 8 bf16).  Row r of fragment u of a group of 64 features is feature 16 (r >> 2) + 4 u + (r & 3) of
+// the group: the accumulators of a lane (point = lane & 15, g = lane >> 4) over the four fragments are
+// then features 16 g .. 16 g + 15, 16 neighbours in memory, whatever the type that is stored.
+#pragma once
+#include "common.h"
+
+#define DEV __device__ __forceinline__
+
+namespace nerf {
+namespace i8 {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+__host__ __device__ inline int64_t up64(int64_t v) { return (v + 63) / 64 * 64; }
+
+constexpr int kMaxWidth = 65536;  // |sum| <= 65536 x 127^2 < 2^31: the int32 sums cannot overflow
+
+struct PackedLayout {
+    int kp, mp;
+    size_t frags, frags_t, bytes;
+    __host__ __device__ PackedLayout(int k, int m, bool with_grad) {
+        kp = (int)up64(k), mp = (int)up64(m);
+        frags = (size_t)mp * 4;
+        frags_t = frags + (size_t)mp * kp;
+        bytes = frags_t + (with_grad ? (size_t)mp * kp * 2 : 0);
+    }
+};
+
+// Feature (inside its group of 64) of row r of fragment u.
+__host__ __device__ inline int frag_feature(int u, int r) { return 16 * (r >> 2) + 4 * u + (r & 3); }
+
+// ---- element types --------------------------------------------------------------------------------
+template <int DT> struct Elem;
+template <> struct Elem<NERF_F32> { typedef float T; };
+template <> struct Elem<NERF_F16> { typedef _Float16 T; };
+template <> struct Elem<NERF_BF16> { typedef __bf16 T; };
+
+inline bool dtype_ok(int dt) { return dt == NERF_F32 || dt == NERF_F16 || dt == NERF_BF16; }
+inline int dtype_size(int dt) { return dt == NERF_F32 ? 4 : 2; }
+
+// N consecutive elements at p (any alignment the element type allows) as floats; only the first `have`
+// exist, the others read as zero.
+template <class T, int N>
+DEV void load_row(const T* p, int have, float (&v)[N]) {
+    if (have >= N) {
+        T t[N];
+        __builtin_memcpy(t, p, sizeof t);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = (float)t[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = i < have ? (float)p[i] : 0.f;
+    }
+}
+
+template <class T, int N>
+DEV void store_row(T* p, int have, const float (&v)[N]) {
+    if (have >= N) {
+        T t[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) t[i] = (T)v[i];
+        __builtin_memcpy(p, t, sizeof t);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i < have) p[i] = (T)v[i];
+    }
+}
+
+// ---- scales ----------------------------------------------------------------------------------------
+// Of a row or channel whose largest magnitude has the bit pattern `top` (a non-negative float orders like
+// its bits; NaN sorts above infinity).  `scale` is what an integer stands for, `inv` what a value is
+// multiplied by before it is rounded.
+//  - power of two: the smallest 2^e >= top / 127, not below 2^-126: rounding is the only loss, and an
+//    integer times its scale is exact in bf16, so that the gradients' products are exact;
+//  - otherwise top / 127: on average 0.7 of the step of the power of two.  Below 2^-100, where the
+//    inverse would overflow, the row is held as zeros;
+//  - infinity or NaN in the row: the scale is NaN, the integers zero; every product of it is NaN.
+struct Scale {
+    float scale, inv;
+};
+DEV Scale scale_of(unsigned top, bool pow2) {
+    if (top >= 0x7f800000u) return {__builtin_bit_cast(float, 0x7fc00000u), 0.f};
+    if (pow2) {
+        int e = (int)(top >> 23) - 133 + ((top & 0x7fffffu) > 0x7e0000u ? 1 : 0);
+        e = e < -126 ? -126 : e;
+        return {__builtin_bit_cast(float, (unsigned)(e + 127) << 23), __builtin_bit_cast(float, (unsigned)(127 - e) << 23)};
+    }
+    if (top < (27u << 23)) return {0.f, 0.f};
+    const float a = __builtin_bit_cast(float, top);
+    return {a / 127.f, 127.f / a};
+}
+DEV unsigned magnitude(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
+// The integer of v: halves to even; a row without a sound scale (inv = 0) gives zeros, NaN included.
+DEV int quantised(float v, float inv) { return inv == 0.f ? 0 : (int)__builtin_rintf(v * inv); }
+
+DEV unsigned pack4(int a, int b, int c, int d) {
+    return (unsigned)(a & 255) | (unsigned)(b & 255) << 8 | (unsigned)(c & 255) << 16 | (unsigned)d << 24;
+}
+
+// ---- bf16 terms -------------------------------------------------------------------------------------
+// How many bf16 numbers a value of a type is the exact sum of (8, 11 and 24 bits of 8 each).
+template <int DT> struct Terms { static constexpr int N = DT == NERF_BF16 ? 1 : DT == NERF_F16 ? 2 : 3; };
+
+// v as the sum of N bf16 terms, each the rounding of what the ones before it leave.  (An infinite v, or one
+// within half a bf16 step of the fp32 maximum, leaves NaN in the second term, so its sums are NaN.)
+template <int N>
+DEV void split_bf16(const float (&v)[8], bf16x8 (&t)[N]) {
+    float rest[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rest[i] = v[i];
+#pragma unroll
+    for (int s = 0; s < N; ++s) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const __bf16 b = (__bf16)rest[i];
+            t[s][i] = b;
+            if (s + 1 < N) rest[i] -= (float)b;
+        }
+    }
+}
+
+}  // namespace i8
+}  // namespace nerf

@@ -391,3 +391,214 @@ def mlp_backward(packed_bwd, act, d_raw, gscale, gbuf, partial, grads, accumulat
         nv.check(nv.lib().nerf_mlp_backward(nv.ptr(packed_bwd), nv.ptr(act), nv.ptr(d_raw), n_points,
                                             float(gscale), nv.ptr(gbuf), nv.ptr(partial), arr,
                                             int(bool(accumulate)), nv.stream()), "nerf_mlp_backward")
+
+
+# ---- dense layers in 8 bits -------------------------------------------------------------------------
+# One layer y = relu(x W + b) of a network that is queried or trained layer by layer (any widths): its
+# input rows are held in 8-bit integers with a scale per row, which the product reads and which is all
+# that is kept for the backward pass; its weights in 8-bit integers with a scale per output channel.
+#
+#     w8 = pack_int8(W, pow2=True)                                   # whenever W changes
+#     rows = quantize_rows(x, pow2=True, want_mask=True)
+#     y = linear_int8(rows, w8, b, relu=True, dtype=torch.bfloat16)  # or linear_int8_quantized: y in 8 bits
+#     dW, db = linear_int8_grad_weight(rows, dz)                     # dz = gradient before this layer's ReLU
+#     dx = linear_int8_grad_input(dz, w8, rows.mask)                 # ... before the ReLU that made x
+#
+# Gradients are those of the product of the 8-bit numbers; rounding to 8 bits passes them on unchanged.
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _padded_width(k):
+    return -(-int(k) // 64) * 64
+
+
+def _on_gpu(what, *tensors):
+    """All given tensors on one GPU -> its device."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise ValueError(f"{what}: expected tensors, got {type(t).__name__}")
+        if not t.is_cuda:
+            raise nv.NerfHipError(f"{what}: expected a tensor on the GPU (the HIP path has no CPU fallback)")
+        if dev is not None and t.device != dev:
+            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+        dev = t.device
+    return dev
+
+
+def _row_major(what, t, width=None):
+    """(tensor, row distance) of a [n, k] tensor of one of the three types whose rows are runs in memory;
+    a tensor with any other strides is copied."""
+    if t.dim() != 2 or t.shape[1] < 1 or (width is not None and t.shape[1] != width):
+        raise ValueError(f"{what}: expected [n, {'k >= 1' if width is None else width}], got {tuple(t.shape)}")
+    if t.dtype not in _DTYPES:
+        raise ValueError(f"{what}: expected float32, float16 or bfloat16, got {t.dtype}")
+    n, k = t.shape
+    if (k > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < k):
+        t = t.contiguous()
+    return t, (max(t.stride(0), k) if n > 1 else k)
+
+
+class Int8Rows:
+    """Rows in 8-bit integers: q [n, k rounded up to 64] int8 with zeros behind column k, scale [n] fp32 (an
+    element is q * scale); pow2: the scales are powers of two (what gradients ask for); mask: None, or
+    the bits x > 0 of the rows as [n, width of q / 8] uint8 (bit f & 7 of byte f >> 3)."""
+
+    __slots__ = ("q", "scale", "k", "pow2", "mask")
+
+    def __init__(self, q, scale, k, pow2=False, mask=None):
+        _on_gpu("Int8Rows", q, scale, mask)
+        k = int(k)
+        if q.dtype != torch.int8 or q.dim() != 2 or k < 1 or q.shape[1] != _padded_width(k):
+            raise ValueError(f"Int8Rows: q must be int8 [n, {_padded_width(k)}] for k = {k}, got {q.dtype} {tuple(q.shape)}")
+        if scale.dtype != torch.float32 or tuple(scale.shape) != (q.shape[0],):
+            raise ValueError(f"Int8Rows: scale must be float32 [{q.shape[0]}], got {scale.dtype} {tuple(scale.shape)}")
+        if mask is not None and (mask.dtype != torch.uint8 or tuple(mask.shape) != (q.shape[0], q.shape[1] // 8)):
+            raise ValueError(f"Int8Rows: mask must be uint8 [{q.shape[0]}, {q.shape[1] // 8}], got {mask.dtype} {tuple(mask.shape)}")
+        if not (q.is_contiguous() and scale.is_contiguous() and (mask is None or mask.is_contiguous())):
+            raise ValueError("Int8Rows: expected contiguous tensors")
+        self.q, self.scale, self.k, self.pow2, self.mask = q, scale, k, bool(pow2), mask
+
+    @property
+    def n(self):
+        return self.q.shape[0]
+
+    def __repr__(self):
+        return f"Int8Rows(n={self.n}, k={self.k}, pow2={self.pow2}, mask={'yes' if self.mask is not None else 'no'})"
+
+
+class Int8Weights:
+    """What pack_int8 returns: the integers and channel scales of W [k, m] as the kernels read them."""
+
+    __slots__ = ("packed", "k", "m", "pow2")
+
+    def __init__(self, packed, k, m, pow2):
+        self.packed, self.k, self.m, self.pow2 = packed, k, m, pow2
+
+    def __repr__(self):
+        return f"Int8Weights(k={self.k}, m={self.m}, pow2={self.pow2})"
+
+
+def _new_rows(n, k, dev, want_mask):
+    kp = _padded_width(k)
+    return (torch.empty((n, kp), dtype=torch.int8, device=dev), torch.empty((n,), dtype=torch.float32, device=dev),
+            torch.empty((n, kp // 8), dtype=torch.uint8, device=dev) if want_mask else None)
+
+
+def quantize_rows(x, pow2=False, want_mask=False):
+    """Int8Rows of x [n, k] (float32, float16 or bfloat16): one scale per row, max|x| / 127 or, with pow2, the
+    next power of two (up to twice the step; rows that a gradient is taken through need it)."""
+    dev = _on_gpu("quantize_rows", x)
+    x, ld = _row_major("quantize_rows", x)
+    n, k = x.shape
+    q, scale, mask = _new_rows(n, k, dev, want_mask)
+    with torch.cuda.device(dev):
+        nv.check(nv.lib().nerf_quantize_rows(ctypes.c_void_p(x.data_ptr()), _DTYPES[x.dtype], n, k, ld, int(bool(pow2)),
+                                             nv.ptr(q), nv.ptr(scale), nv.ptr(mask), nv.stream()), "nerf_quantize_rows")
+    return Int8Rows(q, scale, k, pow2, mask)
+
+
+def pack_int8(w, pow2=False):
+    """Int8Weights of a kernel W [k, m] (fp32, [in, out]): one scale per output channel.  pow2 also lays out
+    what linear_int8_grad_input reads."""
+    dev = _on_gpu("pack_int8", w)
+    if w.dim() != 2 or w.shape[0] < 1 or w.shape[1] < 1:
+        raise ValueError(f"pack_int8: expected [k >= 1, m >= 1], got {tuple(w.shape)}")
+    w = nv.f32(w.detach(), dev)
+    k, m = w.shape
+    need = int(nv.lib().nerf_int8_packed_bytes(k, m, int(bool(pow2))))
+    if need == 0:
+        raise ValueError(f"pack_int8: widths {k} x {m} are beyond what the kernels are built for")
+    packed = torch.empty((need,), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        nv.check(nv.lib().nerf_int8_pack(nv.ptr(w), k, m, int(bool(pow2)), nv.ptr(packed), nv.stream()), "nerf_int8_pack")
+    return Int8Weights(packed, k, m, bool(pow2))
+
+
+def _linear_inputs(what, rows, weights, bias, addend):
+    if not isinstance(rows, Int8Rows) or not isinstance(weights, Int8Weights):
+        raise ValueError(f"{what}: expected Int8Rows and Int8Weights")
+    dev = _on_gpu(what, rows.q, weights.packed, bias, addend)
+    if rows.k != weights.k:
+        raise ValueError(f"{what}: rows of {rows.k} elements against weights for {weights.k}")
+    if bias is not None:
+        bias = nv.f32(bias.detach(), dev)
+        if tuple(bias.shape) != (weights.m,):
+            raise ValueError(f"{what}: bias must be [{weights.m}], got {tuple(bias.shape)}")
+    ldadd, add_dtype = 0, 0
+    if addend is not None:
+        addend, ldadd = _row_major(f"{what} (addend)", addend.detach(), weights.m)
+        add_dtype = _DTYPES[addend.dtype]
+        if addend.shape[0] != rows.n:
+            raise ValueError(f"{what}: addend must have {rows.n} rows, got {addend.shape[0]}")
+    return dev, bias, addend, add_dtype, ldadd
+
+
+def linear_int8(rows, weights, bias=None, relu=False, addend=None, dtype=torch.float32):
+    """y [n, m] = x W (+ bias) (+ addend [n, m]), then relu when asked: the product of the 8-bit integers with
+    exact sums, scaled and finished in fp32, stored in `dtype`."""
+    dev, bias, addend, add_dtype, ldadd = _linear_inputs("linear_int8", rows, weights, bias, addend)
+    if dtype not in _DTYPES:
+        raise ValueError(f"linear_int8: dtype must be float32, float16 or bfloat16, got {dtype}")
+    y = torch.empty((rows.n, weights.m), dtype=dtype, device=dev)
+    with torch.cuda.device(dev):
+        nv.check(nv.lib().nerf_linear_int8(nv.ptr(rows.q), nv.ptr(rows.scale), rows.n, rows.k, nv.ptr(weights.packed),
+                                           weights.m, nv.ptr(bias), None if addend is None else ctypes.c_void_p(addend.data_ptr()),
+                                           add_dtype, ldadd, int(bool(relu)), nv.ptr(y), _DTYPES[dtype], weights.m,
+                                           nv.stream()), "nerf_linear_int8")
+    return y
+
+
+def linear_int8_quantized(rows, weights, bias=None, relu=False, addend=None, pow2=False, want_mask=False):
+    """quantize_rows(linear_int8(...), pow2, want_mask), with y in fp32 in between: the next layer's input."""
+    return quantize_rows(linear_int8(rows, weights, bias, relu, addend), pow2, want_mask)
+
+
+def linear_int8_grad_input(dz, weights, mask=None):
+    """dx [n, k] = dz [n, m] W^T in dz's type, with W as the forward product used it (packed with pow2); zero
+    where `mask` (of the rows that were the layer's input) says that the input was not positive."""
+    what = "linear_int8_grad_input"
+    if not isinstance(weights, Int8Weights):
+        raise ValueError(f"{what}: expected Int8Weights")
+    if not weights.pow2:
+        raise ValueError(f"{what}: weights must be packed with pow2=True")
+    dev = _on_gpu(what, dz, weights.packed, mask)
+    dz, ld = _row_major(what, dz, weights.m)
+    n = dz.shape[0]
+    if mask is not None and (mask.dtype != torch.uint8 or tuple(mask.shape) != (n, _padded_width(weights.k) // 8)):
+        raise ValueError(f"{what}: mask must be uint8 [{n}, {_padded_width(weights.k) // 8}], got {mask.dtype} {tuple(mask.shape)}")
+    dx = torch.empty((n, weights.k), dtype=dz.dtype, device=dev)
+    with torch.cuda.device(dev):
+        nv.check(nv.lib().nerf_linear_int8_grad_input(ctypes.c_void_p(dz.data_ptr()), _DTYPES[dz.dtype], n, weights.m, ld,
+                                                      nv.ptr(weights.packed), weights.k, nv.ptr(mask), nv.ptr(dx), weights.k,
+                                                      nv.stream()), "nerf_linear_int8_grad_input")
+    return dx
+
+
+def linear_int8_grad_weight(rows, dz):
+    """(dW [k, m], db [m]) in fp32 from the rows the forward pass kept (made with pow2) and dz [n, m].  The same
+    inputs give the same bits."""
+    what = "linear_int8_grad_weight"
+    if not isinstance(rows, Int8Rows):
+        raise ValueError(f"{what}: expected Int8Rows")
+    if not rows.pow2:
+        raise ValueError(f"{what}: the rows' scales must be powers of two (quantize_rows(..., pow2=True))")
+    dev = _on_gpu(what, rows.q, dz)
+    dz, ld = _row_major(what, dz)
+    n, m = dz.shape
+    if n != rows.n:
+        raise ValueError(f"{what}: {rows.n} rows against {n} of dz")
+    if n == 0:
+        return (torch.zeros((rows.k, m), dtype=torch.float32, device=dev), torch.zeros((m,), dtype=torch.float32, device=dev))
+    dw = torch.empty((rows.k, m), dtype=torch.float32, device=dev)
+    db = torch.empty((m,), dtype=torch.float32, device=dev)
+    need = int(nv.lib().nerf_linear_int8_grad_weight_bytes(n, rows.k, m))
+    ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+    with torch.cuda.device(dev):
+        nv.check(nv.lib().nerf_linear_int8_grad_weight(nv.ptr(rows.q), nv.ptr(rows.scale), n, rows.k,
+                                                       ctypes.c_void_p(dz.data_ptr()), _DTYPES[dz.dtype], m, ld, nv.ptr(dw),
+                                                       nv.ptr(db), nv.ptr(ws), need, nv.stream()),
+                 "nerf_linear_int8_grad_weight")
+    return dw, db
