@@ -320,6 +320,13 @@ int nerf_linear_int8(const signed char* q, const float* scale, int64_t n, int k,
                      const float* bias, const void* addend, int addend_dtype, int64_t ldadd, int relu,
                      void* y, int dtype, int64_t ldy, nerf_stream_t stream);
 
+/* nerf_quantize_rows of that y (in fp32, never stored): the next layer's rows, yq [n][m rounded up to 64].  For
+ * m up to nerf_linear_int8_quantized_width(k) (256 for k up to 576, else 0); wider: NERF_E_UNSUPPORTED. */
+int nerf_linear_int8_quantized_width(int k);
+int nerf_linear_int8_quantized(const signed char* q, const float* scale, int64_t n, int k, const void* packed, int m,
+                               const float* bias, const void* addend, int addend_dtype, int64_t ldadd, int relu,
+                               int pow2, signed char* yq, float* yscale, unsigned char* ymask, nerf_stream_t stream);
+
 /* dx [n][k] = dz [n][m] times the transposed weights as the forward pass used them (packed with pow2 only:
  * they are then exact in bf16), zero where the bit of `mask` is 0.  dz is taken as the exact sum of 1, 2
  * or 3 bf16 terms (bf16, fp16, fp32): every product is exact, sums are fp32.  dx has dz's type. */

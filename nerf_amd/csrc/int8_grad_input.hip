@@ -1,0 +1,52 @@
+// nerf_linear_int8_grad_input: dz times the transposed weights, which are exact in bf16.
+#include "int8_product.h"
+
+namespace nerf {
+namespace i8 {
+
+constexpr int64_t kResidentRows = 4096;
+
+// Steps of dz rows held in registers: all of 256 columns where they fit beside the sums.
+template <int DT> constexpr int kHeld = DT == NERF_BF16 ? 8 : 4;
+
+template <int DT, int NT>
+static int resident(const LinearArgs& a, const char* what, hipStream_t st) {
+    if (a.steps <= 2) return launch_resident<Bf16Op<DT>, DT, NT, 2>(a, what, st);
+    return launch_resident<Bf16Op<DT>, DT, NT, kHeld<DT>>(a, what, st);
+}
+
+template <int DT>
+static int launch(const LinearArgs& a, const char* what, hipStream_t st) {
+    const int nt = resident_groups(a);
+    if (a.n < kResidentRows || nt == 0) return launch_direct<Bf16Op<DT>, DT>(a, what, st);
+    if (nt == 4) return resident<DT, 4>(a, what, st);
+    if (nt == 2) return resident<DT, 2>(a, what, st);
+    return resident<DT, 1>(a, what, st);
+}
+
+}  // namespace i8
+}  // namespace nerf
+
+using namespace nerf;
+using namespace nerf::i8;
+
+NERF_API int nerf_linear_int8_grad_input(const void* dz, int dtype, int64_t n, int m, int64_t lddz, const void* packed,
+                                         int k, const unsigned char* mask, void* dx, int64_t lddx, nerf_stream_t stream) {
+    const char* what = "nerf_linear_int8_grad_input";
+    if (int rc = require_widths(what, n, k, m)) return rc;
+    NERF_REQUIRE(dtype_ok(dtype), "%s: unknown type %d", what, dtype);
+    if (n == 0) return 0;
+    NERF_REQUIRE(dz && packed && dx, "%s: null pointer", what);
+    NERF_REQUIRE(lddz >= m && lddx >= k, "%s: rows overlap", what);
+    NERF_REQUIRE(((uintptr_t)packed & 15) == 0 && (((uintptr_t)dz | (uintptr_t)dx) & (dtype_size(dtype) - 1)) == 0 &&
+                     ((uintptr_t)mask & 1) == 0,
+                 "%s: misaligned pointer", what);
+    const PackedLayout lay(k, m, true);
+    LinearArgs a{};
+    a.frags = (const char*)packed + lay.frags_t, a.groups = lay.kp / 64, a.steps = lay.mp / 32, a.n = n;
+    a.dz = dz, a.lddz = lddz, a.width = m, a.features = k, a.mask = mask, a.out = dx, a.ldout = lddx;
+    hipStream_t st = as_stream(stream);
+    if (dtype == NERF_F32) return launch<NERF_F32>(a, what, st);
+    if (dtype == NERF_F16) return launch<NERF_F16>(a, what, st);
+    return launch<NERF_BF16>(a, what, st);
+}

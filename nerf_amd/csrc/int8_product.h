@@ -1,0 +1,416 @@
+// Products of rows with packed weights, shared by int8_linear.hip (8-bit integers, int32 sums) and
+// int8_grad_input.hip (bf16 terms, fp32 sums).  Formats: int8_common.h.
+//
+// Both are D[feature][point] = sum over the contraction of A[feature][c] B[c][point] with 16 x 16 tiles:
+// A fragments are stored as the matrix unit takes them, a lane's B fragment is 16 integers (8 bf16)
+// that lie next to each other in its point's row, and the four tiles of a group of 64 features leave
+// 16 neighbouring features of one point in a lane.
+#pragma once
+#include "int8_common.h"
+
+namespace nerf {
+namespace i8 {
+
+struct LinearArgs {
+    const char* frags;     // this product's fragments
+    int groups, steps;     // groups of 64 features, steps of 64 integers (32 bf16)
+    int64_t n;
+    // the rows: q and scale, or dz
+    const signed char* q;
+    const float* scale;
+    const void* dz;
+    int64_t lddz;
+    int width;             // columns of dz (the contraction)
+    // what becomes of the sums
+    int features;          // of a row of the output
+    const float* wscale;
+    const float* bias;
+    const void* addend;    // [n][ldadd] or null
+    int add_dtype;
+    int64_t ldadd;
+    int relu;
+    const unsigned char* mask;
+    void* out;
+    int64_t ldout;
+    // output in 8 bits (TO_INT8): out = integers, and
+    float* out_scale;
+    unsigned char* out_mask;
+    int pow2;
+};
+
+// What a product is stored as: a type (NERF_F32, ...) or 8-bit rows.
+constexpr int TO_INT8 = 3;
+
+// ---- the two products -----------------------------------------------------------------------------
+// Raw: what a lane loads of a point's row for one step; B: the operands made of it.
+struct Int8Op {
+    typedef i32x4 Acc;
+    typedef i32x4 Raw;
+    static constexpr bool kInt8 = true;
+    static DEV Raw fetch(const LinearArgs& a, int64_t p, int s, int g) {
+        return *(const i32x4*)(a.q + (p * a.steps + s) * 64 + 16 * g);
+    }
+    struct B {
+        i32x4 v;
+        DEV B(const Raw& r) : v(r) {}
+    };
+    static DEV Acc mma(i32x4 w, const B& b, Acc c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(w, b.v, c, 0, 0, 0); }
+};
+
+template <int DT>
+struct Bf16Op {
+    typedef f32x4 Acc;
+    typedef typename Elem<DT>::T T;
+    static constexpr bool kInt8 = false;
+    static constexpr int N = Terms<DT>::N;
+    struct Raw {
+        T v[8];
+    };
+    static DEV Raw fetch(const LinearArgs& a, int64_t p, int s, int g) {
+        const int c = 32 * s + 8 * g;
+        const T* src = (const T*)a.dz + p * a.lddz + c;
+        Raw r;
+        if (c + 8 <= a.width) {
+            __builtin_memcpy(r.v, src, sizeof r.v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) r.v[i] = c + i < a.width ? src[i] : (T)0.f;
+        }
+        return r;
+    }
+    struct B {
+        bf16x8 v[N];
+        DEV B(const Raw& r) {
+            if constexpr (DT == NERF_BF16) {
+                __builtin_memcpy(&v[0], r.v, 16);
+            } else {
+                float f[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) f[i] = (float)r.v[i];
+                split_bf16<N>(f, v);
+            }
+        }
+    };
+    static DEV Acc mma(i32x4 w, const B& b, Acc c) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), b.v[i], c, 0, 0, 0);
+        return c;
+    }
+};
+
+// ---- what becomes of the sums of a lane: 16 neighbouring features of point p -------------------------
+DEV void load16(const void* p, int dtype, int64_t at, int have, float (&v)[16]) {
+    if (dtype == NERF_F32) load_row<float, 16>((const float*)p + at, have, v);
+    else if (dtype == NERF_F16) load_row<_Float16, 16>((const _Float16*)p + at, have, v);
+    else load_row<__bf16, 16>((const __bf16*)p + at, have, v);
+}
+
+// A NaN with its sign bit clear, which the integer form of relu keeps; anything else as it is.
+DEV float positive_nan(float v) { return v != v ? __builtin_bit_cast(float, 0x7fc00000u) : v; }
+
+// y = relu((sum x channel scale) x row scale + bias + addend), each step rounded to fp32.  ws, b: the 16
+// channels' scales and biases (0 and 0 behind the last channel; a NaN without its sign).
+DEV void finish_linear(const LinearArgs& a, const i32x4 (&acc)[4], const float* ws, const float* b, float xs, int f, int64_t p,
+                       float (&v)[16]) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const f32x4 w4 = *(const f32x4*)(ws + 4 * u), b4 = *(const f32x4*)(b + 4 * u);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[4 * u + r] = ((float)acc[u][r] * w4[r]) * xs + b4[r];
+    }
+    if (a.addend) {
+        float d[16];
+        load16(a.addend, a.add_dtype, p * a.ldadd + f, a.features - f, d);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = positive_nan(v[i] + d[i]);
+    }
+    if (a.relu) {  // a negative float is a negative integer: one instruction, and a NaN stays one
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int bits = __builtin_bit_cast(int, v[i]);
+            v[i] = __builtin_bit_cast(float, bits > 0 ? bits : 0);
+        }
+    }
+}
+
+template <int DT>
+DEV void store16(const LinearArgs& a, int64_t p, int f, const float (&v)[16]) {
+    typedef typename Elem<DT>::T O;
+    store_row<O, 16>((O*)a.out + p * a.ldout + f, a.features - f, v);
+}
+
+template <int DT>
+DEV void put_grad(const LinearArgs& a, const f32x4 (&acc)[4], int f, int64_t p) {
+    if (f >= a.features) return;
+    unsigned bits = 0xffffu;
+    if (a.mask) bits = *(const unsigned short*)(a.mask + p * (up64(a.features) / 8) + f / 8);
+    float v[16];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[4 * u + r] = bits >> (4 * u + r) & 1 ? acc[u][r] : 0.f;
+    store16<DT>(a, p, f, v);
+}
+
+// Channel scales and biases of `count` features from f0 into LDS, zeros behind the last.
+DEV void stage_channels(const LinearArgs& a, float* ws, float* b, int f0, int count) {
+    for (int i = threadIdx.x; i < count; i += blockDim.x) {
+        const int f = f0 + i;
+        ws[i] = f < a.features ? a.wscale[f] : 0.f;
+        b[i] = (a.bias && f < a.features) ? positive_nan(a.bias[f]) : 0.f;
+    }
+}
+
+// ---- kernels --------------------------------------------------------------------------------------------
+
+// Few rows: one wave per group of 64 features x 32 points, operands straight from global memory.
+template <class Op, int DT>
+__global__ __launch_bounds__(256) void linear_direct_kernel(LinearArgs a) {
+    constexpr int P = 2;
+    __shared__ __attribute__((aligned(16))) float ch[4][2][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, r = lane & 15;
+    const int64_t id = (int64_t)blockIdx.x * 4 + wave;
+    const int T = (int)(id % a.groups);
+    const int64_t p0 = id / a.groups * (16 * P);
+    if (p0 >= a.n) return;
+    typename Op::Acc acc[P][4];
+#pragma unroll
+    for (int j = 0; j < P; ++j)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) acc[j][u] = typename Op::Acc{};
+    int64_t row[P];
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+        const int64_t p = p0 + 16 * j + r;
+        row[j] = p < a.n ? p : a.n - 1;  // a lane behind the last row repeats it and stores nothing
+    }
+    const char* w = a.frags + (size_t)T * a.steps * 4096 + lane * 16;
+    for (int s = 0; s < a.steps; ++s, w += 4096) {
+        typename Op::Raw raw[P];
+#pragma unroll
+        for (int j = 0; j < P; ++j) raw[j] = Op::fetch(a, row[j], s, g);
+        i32x4 wf[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) wf[u] = *(const i32x4*)(w + u * 1024);
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            const typename Op::B b(raw[j]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) acc[j][u] = Op::mma(wf[u], b, acc[j][u]);
+        }
+    }
+    const int f = 64 * T + 16 * g;
+    if constexpr (Op::kInt8) {
+        // this wave's 64 channels, through its own piece of LDS (one wave: in order, no barrier)
+        const int c = 64 * T + lane;
+        ch[wave][0][lane] = c < a.features ? a.wscale[c] : 0.f;
+        ch[wave][1][lane] = (a.bias && c < a.features) ? positive_nan(a.bias[c]) : 0.f;
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            if (p0 + 16 * j + r < a.n && f < a.features) {
+                float v[16];
+                finish_linear(a, acc[j], &ch[wave][0][16 * g], &ch[wave][1][16 * g], a.scale[row[j]], f, row[j], v);
+                store16<DT>(a, row[j], f, v);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < P; ++j)
+            if (p0 + 16 * j + r < a.n) put_grad<DT>(a, acc[j], f, row[j]);
+    }
+}
+
+// Many rows, weights that fit LDS: a workgroup per CU copies the fragments of up to NT groups of
+// features into LDS once and its eight waves then stream tiles of 32 points past them.  A wave holds
+// the sums of all NT groups of a tile (64 NT registers of 32), so a row is read once; the next tile's
+// rows are requested as soon as the last product has read the registers they go to, and arrive
+// behind the work on the sums.  CH steps of rows are held at a time.
+constexpr int kResidentThreads = 512;
+template <int NT>
+constexpr int channel_bytes() { return 2 * NT * 64 * 4; }
+
+template <class Op, int OUT, int NT, int CH>
+__global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(LinearArgs a, int64_t tiles) {
+    constexpr int P = 2;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    float* const ws = (float*)lds;
+    float* const bs = ws + NT * 64;
+    char* const wl = lds + channel_bytes<NT>();
+    const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int T0 = blockIdx.y * NT;
+
+    // fragments [group][step] -> LDS [step][group]; groups behind the last are zeros
+    {
+        const int have = (a.groups - T0 < NT ? a.groups - T0 : NT) * a.steps * 256, all = NT * a.steps * 256;
+        const i32x4* src = (const i32x4*)(a.frags + (size_t)T0 * a.steps * 4096);
+        for (int i = threadIdx.x; i < all; i += kResidentThreads) {
+            const int T = i / (a.steps * 256), s = (i >> 8) - T * a.steps;
+            *(i32x4*)(wl + ((s * NT + T) * 256 + (i & 255)) * 16) = i < have ? src[i] : i32x4{0, 0, 0, 0};
+        }
+        if constexpr (Op::kInt8) stage_channels(a, ws, bs, 64 * T0, NT * 64);
+    }
+    __syncthreads();
+
+    typename Op::Raw raw[CH][P];
+    auto row_of = [&](int64_t tile, int j) {
+        const int64_t p = tile * (16 * P) + 16 * j + r;
+        return p < a.n ? p : a.n - 1;  // a lane behind the last row repeats it and stores nothing
+    };
+    auto fetch = [&](int64_t tile, int s0) {
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            const int64_t p = row_of(tile, j);
+#pragma unroll
+            for (int i = 0; i < CH; ++i)
+                if (s0 + i < a.steps) raw[i][j] = Op::fetch(a, p, s0 + i, g);
+        }
+    };
+    const int64_t stride = (int64_t)gridDim.x * (kResidentThreads / 64);
+    int64_t tile = (int64_t)blockIdx.x * (kResidentThreads / 64) + wave;
+    if (tile < tiles) fetch(tile, 0);
+    for (; tile < tiles; tile += stride) {
+        typename Op::Acc acc[P][NT][4];
+#pragma unroll
+        for (int j = 0; j < P; ++j)
+#pragma unroll
+            for (int T = 0; T < NT; ++T)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) acc[j][T][u] = typename Op::Acc{};
+        for (int s0 = 0; s0 < a.steps; s0 += CH) {
+            if (s0) fetch(tile, s0);
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                if (s0 + i < a.steps) {
+                    const char* w = wl + (s0 + i) * (NT * 4096) + lane * 16;
+                    const typename Op::B b0(raw[i][0]), b1(raw[i][1]);
+#pragma unroll
+                    for (int T = 0; T < NT; ++T)
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            const i32x4 wf = *(const i32x4*)(w + (T * 4 + u) * 1024);
+                            acc[0][T][u] = Op::mma(wf, b0, acc[0][T][u]);
+                            acc[1][T][u] = Op::mma(wf, b1, acc[1][T][u]);
+                        }
+                }
+            }
+        }
+        if (tile + stride < tiles) fetch(tile + stride, 0);
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            const int64_t p = row_of(tile, j);
+            const bool live = tile * (16 * P) + 16 * j + r < a.n;
+            if constexpr (!Op::kInt8) {
+                if (live) {
+#pragma unroll
+                    for (int T = 0; T < NT; ++T) put_grad<OUT>(a, acc[j][T], 64 * (T0 + T) + 16 * g, p);
+                }
+            } else if constexpr (OUT != TO_INT8) {
+                const float xs = a.scale[p];
+#pragma unroll
+                for (int T = 0; T < NT; ++T) {
+                    const int f = 64 * (T0 + T) + 16 * g;
+                    if (live && f < a.features) {
+                        float v[16];
+                        finish_linear(a, acc[j][T], ws + 64 * T + 16 * g, bs + 64 * T + 16 * g, xs, f, p, v);
+                        store16<OUT>(a, p, f, v);
+                    }
+                }
+            } else {
+                // the whole row is here (16 features per group in each of 4 lanes): its scale, then its integers
+                const float xs = a.scale[p];
+                float v[NT][16];
+                unsigned top = 0u;
+#pragma unroll
+                for (int T = 0; T < NT; ++T) {
+                    finish_linear(a, acc[j][T], ws + 64 * T + 16 * g, bs + 64 * T + 16 * g, xs, 64 * T + 16 * g, p, v[T]);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const unsigned m = magnitude(v[T][i]);
+                        top = top > m ? top : m;
+                    }
+                    __builtin_amdgcn_sched_barrier(0);  // in turn: 16 sums become 16 values in the same registers
+                }
+#pragma unroll
+                for (int off = 16; off < 64; off *= 2) {
+                    const unsigned o = (unsigned)__shfl_xor((int)top, off);
+                    top = top > o ? top : o;
+                }
+                const Scale sc = scale_of(top, a.pow2 != 0);
+                const int fp = a.groups * 64;  // width of a row of the output
+                if (live) {
+                    if (g == 0) a.out_scale[p] = sc.scale;
+#pragma unroll
+                    for (int T = 0; T < NT; ++T) {
+                        if (T < a.groups) {
+                            unsigned o[4], bits = 0u;
+#pragma unroll
+                            for (int w = 0; w < 4; ++w) {
+                                int t[4];
+#pragma unroll
+                                for (int b = 0; b < 4; ++b) {
+                                    t[b] = quantised(v[T][4 * w + b], sc.inv);
+                                    bits |= v[T][4 * w + b] > 0.f ? 1u << (4 * w + b) : 0u;
+                                }
+                                o[w] = pack4(t[0], t[1], t[2], t[3]);
+                            }
+                            *(uint4*)((signed char*)a.out + p * fp + 64 * T + 16 * g) = make_uint4(o[0], o[1], o[2], o[3]);
+                            if (a.out_mask) *(unsigned short*)(a.out_mask + p * (fp / 8) + 8 * T + 2 * g) = (unsigned short)bits;
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+            }
+        }
+    }
+}
+
+constexpr int kLdsBytes = 160 * 1024;
+
+template <class Op, int OUT, int NT, int CH>
+int launch_resident(const LinearArgs& a, const char* what, hipStream_t st) {
+    const size_t lds = channel_bytes<NT>() + (size_t)NT * a.steps * 4096;
+    auto kernel = linear_resident_kernel<Op, OUT, NT, CH>;
+    // (the limit is an attribute of the function on every device; asking again costs nothing)
+    const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes);
+    if (e != hipSuccess) return NERF_FAIL((int)e, "%s: %s", what, hipGetErrorString(e));
+    int cus = device_cu_count();
+    if (cus <= 0) cus = 256;
+    const int64_t tiles = (a.n + 31) / 32;
+    const int fblocks = (a.groups + NT - 1) / NT;
+    int64_t blocks = (tiles + kResidentThreads / 64 - 1) / (kResidentThreads / 64);
+    const int64_t most = cus / fblocks > 0 ? cus / fblocks : 1;
+    if (blocks > most) blocks = most;
+    kernel<<<dim3((unsigned)blocks, (unsigned)fblocks), kResidentThreads, lds, st>>>(a, tiles);
+    return check_launch(what);
+}
+
+template <class Op, int DT>
+int launch_direct(const LinearArgs& a, const char* what, hipStream_t st) {
+    const int64_t waves = (a.n + 31) / 32 * a.groups;
+    if ((waves + 3) / 4 >= (1LL << 24)) return NERF_FAIL(NERF_E_UNSUPPORTED, "%s: too many rows", what);
+    linear_direct_kernel<Op, DT><<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(a);
+    return check_launch(what);
+}
+
+inline int require_widths(const char* what, int64_t n, int k, int m) {
+    NERF_REQUIRE(n >= 0 && k >= 1 && m >= 1 && k <= kMaxWidth && m <= kMaxWidth, "%s: bad size (%lld rows, %d x %d)", what, (long long)n, k, m);
+    return 0;
+}
+
+// Groups of features a workgroup of the resident kernel holds: as few feature blocks as LDS allows (each
+// reads the rows again), the groups spread evenly over them; 0: not even one group fits.
+inline int resident_groups(const LinearArgs& a) {
+    int most = (kLdsBytes - channel_bytes<4>()) / (a.steps * 4096);
+    if (most > 4) most = 4;
+    if (most < 1) return 0;
+    const int blocks = (a.groups + most - 1) / most;
+    int nt = (a.groups + blocks - 1) / blocks;
+    if (nt == 3 && most < 4) nt = 2;
+    return nt == 3 ? 4 : nt;
+}
+
+}  // namespace i8
+}  // namespace nerf

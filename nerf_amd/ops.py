@@ -552,8 +552,19 @@ def linear_int8(rows, weights, bias=None, relu=False, addend=None, dtype=torch.f
 
 
 def linear_int8_quantized(rows, weights, bias=None, relu=False, addend=None, pow2=False, want_mask=False):
-    """quantize_rows(linear_int8(...), pow2, want_mask), with y in fp32 in between: the next layer's input."""
-    return quantize_rows(linear_int8(rows, weights, bias, relu, addend), pow2, want_mask)
+    """quantize_rows(linear_int8(...), pow2, want_mask), with y in fp32 in between: the next layer's input.  One
+    kernel that never stores y for up to 256 outputs of up to 576 inputs; the two calls otherwise."""
+    dev, bias, addend, add_dtype, ldadd = _linear_inputs("linear_int8_quantized", rows, weights, bias, addend)
+    if weights.m > nv.lib().nerf_linear_int8_quantized_width(rows.k):
+        return quantize_rows(linear_int8(rows, weights, bias, relu, addend), pow2, want_mask)
+    q, scale, mask = _new_rows(rows.n, weights.m, dev, want_mask)
+    with torch.cuda.device(dev):
+        nv.check(nv.lib().nerf_linear_int8_quantized(nv.ptr(rows.q), nv.ptr(rows.scale), rows.n, rows.k, nv.ptr(weights.packed),
+                                                     weights.m, nv.ptr(bias),
+                                                     None if addend is None else ctypes.c_void_p(addend.data_ptr()), add_dtype,
+                                                     ldadd, int(bool(relu)), int(bool(pow2)), nv.ptr(q), nv.ptr(scale),
+                                                     nv.ptr(mask), nv.stream()), "nerf_linear_int8_quantized")
+    return Int8Rows(q, scale, weights.m, pow2, mask)
 
 
 def linear_int8_grad_input(dz, weights, mask=None):

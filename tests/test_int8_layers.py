@@ -13,7 +13,8 @@ TYPES = {"float32": torch.float32, "float16": torch.float16, "bfloat16": torch.b
 TERMS = {torch.float32: 3, torch.float16: 2, torch.bfloat16: 1}   # bf16 terms of an element of dz
 TINY = {t: max(torch.finfo(t).smallest_normal * torch.finfo(t).eps, 1e-38) for t in TERMS}   # below the normal numbers: a step
 SHAPES = [(1, 1, 1), (1, 256, 256), (3, 63, 5), (17, 64, 64), (31, 65, 63), (33, 128, 3), (64, 319, 256), (257, 283, 128),
-          (1000, 27, 129), (130, 2048, 17), (65, 130, 700), (4100, 256, 256), (129, 600, 1), (16, 2047, 33)]
+          (1000, 27, 129), (130, 2048, 17), (65, 130, 700), (4100, 256, 256), (129, 600, 1), (16, 2047, 33),
+          (4111, 63, 256), (4099, 283, 128), (5003, 319, 256), (4097, 128, 3), (6001, 27, 70), (4133, 700, 200), (4100, 1100, 65), (33000, 256, 192), (70001, 64, 64)]
 
 
 # ---- without a GPU -----------------------------------------------------------------------------------
@@ -45,6 +46,13 @@ def test_bad_arguments_are_refused_without_a_gpu():
                 dict(dt=5), dict(ldy=7), dict(addend=one, ldadd=7), dict(addend=one, ldadd=8, adt=9), dict(bias=odd), dict(y=odd)):
         assert linear(**bad) == -1, bad
     assert linear(n=0, q=None) == 0
+    assert lib.nerf_linear_int8_quantized_width(576) == 256 and lib.nerf_linear_int8_quantized_width(577) == 0
+    quant = lambda **c: lib.nerf_linear_int8_quantized(*[{**dict(q=one, scale=one, n=4, k=8, packed=one, m=8, bias=None, addend=None, adt=0, ldadd=0,
+                                                                 relu=0, pow2=0, yq=one, ys=one, ym=None, st=None), **c}[x] for x in
+                                                         ("q", "scale", "n", "k", "packed", "m", "bias", "addend", "adt", "ldadd", "relu", "pow2", "yq", "ys", "ym", "st")])
+    for bad in (dict(q=None), dict(yq=None), dict(ys=None), dict(yq=odd), dict(ym=odd), dict(k=0), dict(m=0), dict(n=-1), dict(addend=one, ldadd=7)):
+        assert quant(**bad) == -1, bad
+    assert quant(m=257) == -2 and quant(k=577) == -2
     gi = lambda **c: lib.nerf_linear_int8_grad_input(*[{**dict(dz=one, dt=0, n=4, m=8, lddz=8, packed=one, k=8, mask=None, dx=one, lddx=8, st=None), **c}[x]
                                                        for x in ("dz", "dt", "n", "m", "lddz", "packed", "k", "mask", "dx", "lddx", "st")])
     for bad in (dict(dz=None), dict(dx=None), dict(packed=odd), dict(dt=3), dict(lddz=7), dict(lddx=7), dict(mask=odd), dict(k=0), dict(n=-1)):
