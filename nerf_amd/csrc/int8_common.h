@@ -56,6 +56,152 @@ template <> struct Elem<NERF_BF16> { typedef __bf16 T; };
 inline bool dtype_ok(int dt) { return dt == NERF_F32 || dt == NERF_F16 || dt == NERF_BF16; }
 inline int dtype_size(int dt) { return dt == NERF_F32 ? 4 : 2; }
 
+// 16 bytes at any address that the element type allows (global memory takes unaligned vectors).
+typedef int i32x4u __attribute__((ext_vector_type(4), aligned(2)));
+typedef int i32x2u __attribute__((ext_vector_type(2), aligned(2)));
+typedef int i32u __attribute__((aligned(2)));
+
+// Eight neighbouring elements as they are loaded: one register quad of 16-bit elements, or two of fp32.
+template <class T> struct Raw8 {
+    i32x4 w[sizeof(T) / 2 == 1 ? 1 : 2];
+};
+
+template <class T>
+DEV void to_float(const Raw8<T>& r, float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int w = r.w[i >> 2][i & 3];  // (a bit cast of a vector's element itself takes element 0)
+            v[i] = __builtin_bit_cast(float, w);
+        }
+    } else if constexpr (__is_same(T, __bf16)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __builtin_bit_cast(float, r.w[0][i] << 16);
+            v[2 * i + 1] = __builtin_bit_cast(float, r.w[0][i] & (int)0xffff0000);
+        }
+    } else {
+        typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+        const half8 h = __builtin_bit_cast(half8, r.w[0]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)h[i];
+    }
+}
+
+// Elements c .. c + 7 of a row of `width`; those behind its end are zero.  `whole` (the same in every lane):
+// no lane's piece passes the end.  A piece that does is read so that it ends with the row, and shifted
+// down: three steps of selects instead of eight guarded loads.
+template <class T>
+DEV Raw8<T> load8(const T* row, int c, int width, bool whole) {
+    Raw8<T> r;
+    constexpr int W = sizeof(T) == 4 ? 8 : 4;  // words of a piece
+    if (whole) {
+#pragma unroll
+        for (int i = 0; i < W / 4; ++i) r.w[i] = *(const i32x4u*)((const char*)(row + c) + 16 * i);
+        return r;
+    }
+    int w[W];
+    if (width >= 8) {
+        const int over = c + 8 - width;  // elements behind the end
+        const T* src = row + (over > 0 ? width - 8 : c);
+#pragma unroll
+        for (int i = 0; i < W / 4; ++i) {
+            const i32x4 q = *(const i32x4u*)((const char*)src + 16 * i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[4 * i + j] = q[j];
+        }
+        const int e = over < 0 ? 0 : over;
+        if constexpr (W == 8) {
+#pragma unroll
+            for (int k = 4; k >= 1; k /= 2)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[i] = (e & k) ? (i + k < 8 ? w[i + k] : 0) : w[i];
+        } else {
+#pragma unroll
+            for (int k = 2; k >= 1; k /= 2)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = (e & (2 * k)) ? (i + k < 4 ? w[i + k] : 0) : w[i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = (e & 1) ? (int)((unsigned)w[i] >> 16 | (i < 3 ? (unsigned)w[i + 1] << 16 : 0u)) : w[i];
+        }
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = e >= 8 ? 0 : w[i];
+    } else {  // a row shorter than a piece
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            if constexpr (W == 8) {
+                w[i] = c + i < width ? __builtin_bit_cast(int, row[c + i]) : 0;
+            } else {
+                const unsigned lo = c + 2 * i < width ? __builtin_bit_cast(unsigned short, row[c + 2 * i]) : 0;
+                const unsigned hi = c + 2 * i + 1 < width ? __builtin_bit_cast(unsigned short, row[c + 2 * i + 1]) : 0;
+                w[i] = (int)(lo | hi << 16);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) r.w[i >> 2][i & 3] = w[i];
+    return r;
+}
+
+// Elements f .. f + 15 of a row of `width`, as far as they exist; `whole` as above.  A piece that passes the
+// end leaves as runs of 8, 4, 2 and 1 elements.
+template <class T>
+DEV void store16(T* row, int f, int width, bool whole, const float (&v)[16]) {
+    constexpr int W = sizeof(T) == 4 ? 16 : 8;
+    int w[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        if constexpr (W == 16) {
+            w[i] = __builtin_bit_cast(int, v[i]);
+        } else {
+            typedef T pair __attribute__((ext_vector_type(2)));
+            const pair t = {(T)v[2 * i], (T)v[2 * i + 1]};
+            w[i] = __builtin_bit_cast(int, t);
+        }
+    }
+    char* dst = (char*)(row + f);
+    if (whole || f + 16 <= width) {
+#pragma unroll
+        for (int i = 0; i < W / 4; ++i) *(i32x4u*)(dst + 16 * i) = i32x4{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+        return;
+    }
+    const int have = width - f;
+    if (have <= 0) return;
+    constexpr int kRun8 = W / 2;  // words of 8 elements
+    if (have & 8) {
+#pragma unroll
+        for (int i = 0; i < kRun8 / 4; ++i) *(i32x4u*)(dst + 16 * i) = i32x4{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+        dst += 4 * kRun8;
+#pragma unroll
+        for (int i = 0; i < kRun8; ++i) w[i] = w[i + kRun8];
+    }
+    if constexpr (W == 16) {
+        if (have & 4) {
+            *(i32x4u*)dst = i32x4{w[0], w[1], w[2], w[3]};
+            dst += 16;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = w[i + 4];
+        }
+        if (have & 2) {
+            typedef int i32x2 __attribute__((ext_vector_type(2)));
+            *(i32x2u*)dst = i32x2{w[0], w[1]};
+            dst += 8, w[0] = w[2];
+        }
+        if (have & 1) *(i32u*)dst = w[0];
+    } else {
+        if (have & 4) {
+            typedef int i32x2 __attribute__((ext_vector_type(2)));
+            *(i32x2u*)dst = i32x2{w[0], w[1]};
+            dst += 8, w[0] = w[2], w[1] = w[3];
+        }
+        if (have & 2) {
+            *(i32u*)dst = w[0];
+            dst += 4, w[0] = w[1];
+        }
+        if (have & 1) *(unsigned short*)dst = (unsigned short)w[0];
+    }
+}
+
 // N consecutive elements at p (any alignment the element type allows) as floats; only the first `have`
 // exist, the others read as zero.
 template <class T, int N>
@@ -68,20 +214,6 @@ DEV void load_row(const T* p, int have, float (&v)[N]) {
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = i < have ? (float)p[i] : 0.f;
-    }
-}
-
-template <class T, int N>
-DEV void store_row(T* p, int have, const float (&v)[N]) {
-    if (have >= N) {
-        T t[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) t[i] = (T)v[i];
-        __builtin_memcpy(p, t, sizeof t);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (i < have) p[i] = (T)v[i];
     }
 }
 
@@ -114,6 +246,17 @@ DEV int quantised(float v, float inv) { return inv == 0.f ? 0 : (int)__builtin_r
 
 DEV unsigned pack4(int a, int b, int c, int d) {
     return (unsigned)(a & 255) | (unsigned)(b & 255) << 8 | (unsigned)(c & 255) << 16 | (unsigned)d << 24;
+}
+
+// Four finite numbers of magnitude at most 127.5 rounded to bytes, halves to even: added to 1.5 x 2^23, where
+// a float's step is 1, they leave the integer in its low byte (one addition instead of a rounding and
+// a conversion, and a byte permutation instead of masks and shifts).
+DEV unsigned round4(const float (&t)[4]) {
+    unsigned b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = __builtin_bit_cast(unsigned, t[i] + 12582912.f);
+    const unsigned lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u);
+    return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
 }
 
 // ---- bf16 terms -------------------------------------------------------------------------------------

@@ -7,18 +7,19 @@ namespace i8 {
 constexpr int64_t kResidentRows = 4096;
 
 // Steps of dz rows held in registers: all of 256 columns where they fit beside the sums.
-template <int DT> constexpr int kHeld = DT == NERF_BF16 ? 8 : 4;
+template <int DT> constexpr int kHeld = DT == NERF_BF16 ? 8 : DT == NERF_F16 ? 4 : 3;
 
 template <int DT, int NT>
 static int resident(const LinearArgs& a, const char* what, hipStream_t st) {
-    if (a.steps <= 2) return launch_resident<Bf16Op<DT>, DT, NT, 2>(a, what, st);
-    return launch_resident<Bf16Op<DT>, DT, NT, kHeld<DT>>(a, what, st);
+    if (a.width % 32 != 0) return launch_resident<Bf16Op<DT, false>, DT, NT, 2, false>(a, what, st);
+    if (a.steps <= 2) return launch_resident<Bf16Op<DT, true>, DT, NT, 2, false>(a, what, st);
+    return launch_resident<Bf16Op<DT, true>, DT, NT, kHeld<DT>, false>(a, what, st);
 }
 
 template <int DT>
 static int launch(const LinearArgs& a, const char* what, hipStream_t st) {
     const int nt = resident_groups(a);
-    if (a.n < kResidentRows || nt == 0) return launch_direct<Bf16Op<DT>, DT>(a, what, st);
+    if (a.n < kResidentRows || nt == 0) return launch_direct<Bf16Op<DT, false>, DT, false>(a, what, st);
     if (nt == 4) return resident<DT, 4>(a, what, st);
     if (nt == 2) return resident<DT, 2>(a, what, st);
     return resident<DT, 1>(a, what, st);

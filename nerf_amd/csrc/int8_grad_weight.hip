@@ -48,6 +48,7 @@ __global__ __launch_bounds__(256) void grad_weight_kernel(GradWeightArgs a) {
     constexpr int kChunks = MT >= 64 ? MT / 64 : 1;   // pieces of 8 features of dz per thread and stage
     constexpr int kStage = (XT + N * YT) * kImg;
     constexpr int AX = MT == 32 ? 1 : 2, AY = MT == 32 ? 1 : 2;  // 32 x 32 tiles of a wave
+    constexpr int D = DT == NERF_F32 ? 2 : 4;  // even: the LDS buffer of a turn is then known when compiling
     static_assert(MT == 32 || MT == 128, "tile");
     __shared__ __attribute__((aligned(16))) char lds[2 * kStage];
 
@@ -69,51 +70,57 @@ __global__ __launch_bounds__(256) void grad_weight_kernel(GradWeightArgs a) {
     const int yq = t & 3, yp = (t >> 2) & 31, yt0 = t >> 7;
     const bool has_y = MT >= 64 || t < 128;
 
-    i32x4 xr;
-    T yr[kChunks][8];
-    float sr;
+    const int xc = xcol < a.kp ? xcol : 0;   // columns behind the last are computed and not stored
+    const bool y_whole = mb * MT + MT <= a.m;
+
+    // Stages D - 1 turns ahead are on their way in registers: one stage of a workgroup is only some 12 KiB.
+    struct Held {
+        i32x4 x;
+        Raw8<T> y[kChunks];
+        float s;
+    };
+    Held held[D];
     float sum[kChunks][8];
 #pragma unroll
     for (int i = 0; i < kChunks; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum[i][j] = 0.f;
 
-    auto fetch = [&](int64_t st) {
+    auto fetch = [&](int64_t st, Held& h) {
         const int64_t row0 = lo + st * kStageRows;
-        xr = i32x4{0, 0, 0, 0};
-        if (row0 + xp < hi && xcol < a.kp) xr = *(const i32x4*)(a.q + (row0 + xp) * a.kp + xcol);
-        const int64_t row = row0 + yp;
-        const bool on = has_y && row < hi;
-        sr = on ? a.scale[row] : 0.f;
+        const int64_t rx = row0 + xp < hi ? row0 + xp : hi - 1;   // a row behind the last: its dz is taken as zero
+        h.x = *(const i32x4*)(a.q + rx * a.kp + xc);
+        if (has_y) {
+            const int64_t ry = row0 + yp < hi ? row0 + yp : hi - 1;
+            h.s = a.scale[ry];
+            const T* src = (const T*)a.dz + ry * a.lddz;
 #pragma unroll
-        for (int i = 0; i < kChunks; ++i) {
-            const int col = mb * MT + (yt0 + 2 * i) * 32 + yq * 8;
-            const T* src = (const T*)a.dz + row * a.lddz + col;
-            if (on && col + 8 <= a.m) {
-                __builtin_memcpy(yr[i], src, sizeof yr[i]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) yr[i][j] = (on && col + j < a.m) ? src[j] : (T)0.f;
-            }
+            for (int i = 0; i < kChunks; ++i) h.y[i] = load8<T>(src, mb * MT + (yt0 + 2 * i) * 32 + yq * 8, a.m, y_whole);
         }
     };
-    auto stage = [&](char* buf) {
+    auto stage = [&](int64_t st, const Held& h, char* buf) {
         {
             bf16x8 o[2];
 #pragma unroll
             for (int w = 0; w < 4; ++w)
 #pragma unroll
-                for (int b = 0; b < 4; ++b) o[w >> 1][(w & 1) * 4 + b] = (__bf16)(float)((xr[w] << (24 - 8 * b)) >> 24);
+                for (int b = 0; b < 4; ++b) o[w >> 1][(w & 1) * 4 + b] = (__bf16)(float)((h.x[w] << (24 - 8 * b)) >> 24);
             char* dst = buf + xt * kImg + xp * 64 + xh * 32;
             *(bf16x8*)dst = o[0];
             *(bf16x8*)(dst + 16) = o[1];
         }
         if (has_y) {
+            const bool on = lo + st * kStageRows + yp < hi;
 #pragma unroll
             for (int i = 0; i < kChunks; ++i) {
                 float v[8];
+                to_float(h.y[i], v);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = (float)yr[i][j], sum[i][j] += v[j], v[j] *= sr;
+                for (int j = 0; j < 8; ++j) {
+                    v[j] = on ? v[j] : 0.f;
+                    sum[i][j] += v[j];
+                    v[j] *= on ? h.s : 0.f;
+                }
                 bf16x8 o[N];
                 split_bf16<N>(v, o);
 #pragma unroll
@@ -132,30 +139,36 @@ __global__ __launch_bounds__(256) void grad_weight_kernel(GradWeightArgs a) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
 
-    if (stages > 0) {
-        fetch(0);
-        stage(lds);
-    }
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+        if (d < stages) fetch(d, held[d]);
+    if (stages > 0) stage(0, held[0], lds);
     __syncthreads();
-    for (int64_t st = 0; st < stages; ++st) {
-        const char* buf = lds + (st & 1) * kStage;
-        if (st + 1 < stages) fetch(st + 1);
+    for (int64_t st0 = 0; st0 < stages; st0 += D) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            bf16x8 xo[AX];
+        for (int d = 0; d < D; ++d) {
+            const int64_t st = st0 + d;
+            if (st >= stages) break;
+            const char* buf = lds + (d & 1) * kStage;
+            if (st + D < stages) fetch(st + D, held[d]);
 #pragma unroll
-            for (int x = 0; x < AX; ++x) xo[x] = tr_operand(buf + (wx + x) * kImg, half, lane);
+            for (int half = 0; half < 2; ++half) {
+                bf16x8 xo[AX];
 #pragma unroll
-            for (int s = 0; s < N; ++s)
+                for (int x = 0; x < AX; ++x) xo[x] = tr_operand(buf + (wx + x) * kImg, half, lane);
 #pragma unroll
-                for (int y = 0; y < AY; ++y) {
-                    const bf16x8 yo = tr_operand(buf + (XT + s * YT + wy + y) * kImg, half, lane);
+                for (int s = 0; s < N; ++s)
 #pragma unroll
-                    for (int x = 0; x < AX; ++x) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xo[x], yo, acc[x][y], 0, 0, 0);
-                }
+                    for (int y = 0; y < AY; ++y) {
+                        const bf16x8 yo = tr_operand(buf + (XT + s * YT + wy + y) * kImg, half, lane);
+#pragma unroll
+                        for (int x = 0; x < AX; ++x) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xo[x], yo, acc[x][y], 0, 0, 0);
+                    }
+            }
+            // into the buffer that was read in the turn before this one
+            if (st + 1 < stages) stage(st + 1, held[(d + 1) % D], lds + ((d + 1) & 1) * kStage);
+            __syncthreads();
         }
-        if (st + 1 < stages) stage(lds + ((st + 1) & 1) * kStage);  // read last in the turn before this one
-        __syncthreads();
     }
 
     float* out = a.out + slice * a.stride;

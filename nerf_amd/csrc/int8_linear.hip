@@ -7,22 +7,26 @@ namespace i8 {
 // Rows from which the resident kernel's copy of the weights into every CU pays.
 constexpr int64_t kResidentRows = 4096;
 
-template <int OUT, int NT>
+template <int OUT, int NT, bool ADD>
 static int resident(const LinearArgs& a, const char* what, hipStream_t st) {
-    if (a.steps == 1) return launch_resident<Int8Op, OUT, NT, 1>(a, what, st);
-    if (a.steps == 2) return launch_resident<Int8Op, OUT, NT, 2>(a, what, st);
-    return launch_resident<Int8Op, OUT, NT, 5>(a, what, st);
+    if (a.steps <= 2) return launch_resident<Int8Op, OUT, NT, 2, ADD>(a, what, st);
+    return launch_resident<Int8Op, OUT, NT, 5, ADD>(a, what, st);
+}
+
+template <int OUT, bool ADD>
+static int launch(const LinearArgs& a, const char* what, hipStream_t st) {
+    const int nt = resident_groups(a);
+    if constexpr (OUT != TO_INT8) {
+        if (a.n < kResidentRows || nt == 0) return launch_direct<Int8Op, OUT, ADD>(a, what, st);
+    }
+    if (nt == 4) return resident<OUT, 4, ADD>(a, what, st);
+    if (nt == 2) return resident<OUT, 2, ADD>(a, what, st);
+    return resident<OUT, 1, ADD>(a, what, st);
 }
 
 template <int OUT>
 static int launch(const LinearArgs& a, const char* what, hipStream_t st) {
-    const int nt = resident_groups(a);
-    if constexpr (OUT != TO_INT8) {
-        if (a.n < kResidentRows || nt == 0) return launch_direct<Int8Op, OUT>(a, what, st);
-    }
-    if (nt == 4) return resident<OUT, 4>(a, what, st);
-    if (nt == 2) return resident<OUT, 2>(a, what, st);
-    return resident<OUT, 1>(a, what, st);
+    return a.addend ? launch<OUT, true>(a, what, st) : launch<OUT, false>(a, what, st);
 }
 
 // Checks and fields that both entry points share.

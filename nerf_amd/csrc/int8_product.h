@@ -57,36 +57,25 @@ struct Int8Op {
     static DEV Acc mma(i32x4 w, const B& b, Acc c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(w, b.v, c, 0, 0, 0); }
 };
 
-template <int DT>
+// EVEN: the rows of dz end with a step (32 columns), so that no piece of one needs the care of a ragged end.
+template <int DT, bool EVEN>
 struct Bf16Op {
     typedef f32x4 Acc;
     typedef typename Elem<DT>::T T;
+    typedef Raw8<T> Raw;
     static constexpr bool kInt8 = false;
     static constexpr int N = Terms<DT>::N;
-    struct Raw {
-        T v[8];
-    };
     static DEV Raw fetch(const LinearArgs& a, int64_t p, int s, int g) {
-        const int c = 32 * s + 8 * g;
-        const T* src = (const T*)a.dz + p * a.lddz + c;
-        Raw r;
-        if (c + 8 <= a.width) {
-            __builtin_memcpy(r.v, src, sizeof r.v);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) r.v[i] = c + i < a.width ? src[i] : (T)0.f;
-        }
-        return r;
+        return load8<T>((const T*)a.dz + p * a.lddz, 32 * s + 8 * g, a.width, EVEN || 32 * s + 32 <= a.width);
     }
     struct B {
         bf16x8 v[N];
         DEV B(const Raw& r) {
             if constexpr (DT == NERF_BF16) {
-                __builtin_memcpy(&v[0], r.v, 16);
+                v[0] = __builtin_bit_cast(bf16x8, r.w[0]);
             } else {
                 float f[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) f[i] = (float)r.v[i];
+                to_float(r, f);
                 split_bf16<N>(f, v);
             }
         }
@@ -100,10 +89,15 @@ struct Bf16Op {
 };
 
 // ---- what becomes of the sums of a lane: 16 neighbouring features of point p -------------------------
-DEV void load16(const void* p, int dtype, int64_t at, int have, float (&v)[16]) {
-    if (dtype == NERF_F32) load_row<float, 16>((const float*)p + at, have, v);
-    else if (dtype == NERF_F16) load_row<_Float16, 16>((const _Float16*)p + at, have, v);
-    else load_row<__bf16, 16>((const __bf16*)p + at, have, v);
+template <class T>
+DEV void add16(const T* row, int f, int width, bool whole, float (&v)[16]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float d[8];
+        to_float(load8<T>(row, f + 8 * h, width, whole), d);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[8 * h + i] += d[i];
+    }
 }
 
 // A NaN with its sign bit clear, which the integer form of relu keeps; anything else as it is.
@@ -111,19 +105,21 @@ DEV float positive_nan(float v) { return v != v ? __builtin_bit_cast(float, 0x7f
 
 // y = relu((sum x channel scale) x row scale + bias + addend), each step rounded to fp32.  ws, b: the 16
 // channels' scales and biases (0 and 0 behind the last channel; a NaN without its sign).
+template <bool ADD>
 DEV void finish_linear(const LinearArgs& a, const i32x4 (&acc)[4], const float* ws, const float* b, float xs, int f, int64_t p,
-                       float (&v)[16]) {
+                       bool whole, float (&v)[16]) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
         const f32x4 w4 = *(const f32x4*)(ws + 4 * u), b4 = *(const f32x4*)(b + 4 * u);
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[4 * u + r] = ((float)acc[u][r] * w4[r]) * xs + b4[r];
     }
-    if (a.addend) {
-        float d[16];
-        load16(a.addend, a.add_dtype, p * a.ldadd + f, a.features - f, d);
+    if constexpr (ADD) {
+        if (a.add_dtype == NERF_F32) add16((const float*)a.addend + p * a.ldadd, f, a.features, whole, v);
+        else if (a.add_dtype == NERF_F16) add16((const _Float16*)a.addend + p * a.ldadd, f, a.features, whole, v);
+        else add16((const __bf16*)a.addend + p * a.ldadd, f, a.features, whole, v);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = positive_nan(v[i] + d[i]);
+        for (int i = 0; i < 16; ++i) v[i] = positive_nan(v[i]);
     }
     if (a.relu) {  // a negative float is a negative integer: one instruction, and a NaN stays one
 #pragma unroll
@@ -135,22 +131,24 @@ DEV void finish_linear(const LinearArgs& a, const i32x4 (&acc)[4], const float* 
 }
 
 template <int DT>
-DEV void store16(const LinearArgs& a, int64_t p, int f, const float (&v)[16]) {
+DEV void put(const LinearArgs& a, int64_t p, int f, bool whole, const float (&v)[16]) {
     typedef typename Elem<DT>::T O;
-    store_row<O, 16>((O*)a.out + p * a.ldout + f, a.features - f, v);
+    store16<O>((O*)a.out + p * a.ldout, f, a.features, whole, v);
+}
+
+// Bits of the mask of features f .. f + 15 of point p (rows of bits are padded like rows of integers).
+DEV unsigned mask_bits(const LinearArgs& a, int64_t p, int f) {
+    return a.mask ? *(const unsigned short*)(a.mask + p * (a.groups * 8) + f / 8) : 0xffffu;
 }
 
 template <int DT>
-DEV void put_grad(const LinearArgs& a, const f32x4 (&acc)[4], int f, int64_t p) {
-    if (f >= a.features) return;
-    unsigned bits = 0xffffu;
-    if (a.mask) bits = *(const unsigned short*)(a.mask + p * (up64(a.features) / 8) + f / 8);
+DEV void put_grad(const LinearArgs& a, const f32x4 (&acc)[4], int f, int64_t p, bool whole, unsigned bits) {
     float v[16];
 #pragma unroll
     for (int u = 0; u < 4; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[4 * u + r] = bits >> (4 * u + r) & 1 ? acc[u][r] : 0.f;
-    store16<DT>(a, p, f, v);
+    put<DT>(a, p, f, whole, v);
 }
 
 // Channel scales and biases of `count` features from f0 into LDS, zeros behind the last.
@@ -165,7 +163,7 @@ DEV void stage_channels(const LinearArgs& a, float* ws, float* b, int f0, int co
 // ---- kernels --------------------------------------------------------------------------------------------
 
 // Few rows: one wave per group of 64 features x 32 points, operands straight from global memory.
-template <class Op, int DT>
+template <class Op, int DT, bool ADD>
 __global__ __launch_bounds__(256) void linear_direct_kernel(LinearArgs a) {
     constexpr int P = 2;
     __shared__ __attribute__((aligned(16))) float ch[4][2][64];
@@ -201,6 +199,7 @@ __global__ __launch_bounds__(256) void linear_direct_kernel(LinearArgs a) {
         }
     }
     const int f = 64 * T + 16 * g;
+    const bool whole = 64 * T + 64 <= a.features;
     if constexpr (Op::kInt8) {
         // this wave's 64 channels, through its own piece of LDS (one wave: in order, no barrier)
         const int c = 64 * T + lane;
@@ -209,16 +208,14 @@ __global__ __launch_bounds__(256) void linear_direct_kernel(LinearArgs a) {
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int j = 0; j < P; ++j) {
-            if (p0 + 16 * j + r < a.n && f < a.features) {
-                float v[16];
-                finish_linear(a, acc[j], &ch[wave][0][16 * g], &ch[wave][1][16 * g], a.scale[row[j]], f, row[j], v);
-                store16<DT>(a, row[j], f, v);
-            }
+            float v[16];
+            finish_linear<ADD>(a, acc[j], &ch[wave][0][16 * g], &ch[wave][1][16 * g], a.scale[row[j]], f, row[j], whole, v);
+            if (p0 + 16 * j + r < a.n) put<DT>(a, row[j], f, whole, v);
         }
     } else {
 #pragma unroll
         for (int j = 0; j < P; ++j)
-            if (p0 + 16 * j + r < a.n) put_grad<DT>(a, acc[j], f, row[j]);
+            if (p0 + 16 * j + r < a.n) put_grad<DT>(a, acc[j], f, row[j], whole, mask_bits(a, row[j], f));
     }
 }
 
@@ -231,7 +228,7 @@ constexpr int kResidentThreads = 512;
 template <int NT>
 constexpr int channel_bytes() { return 2 * NT * 64 * 4; }
 
-template <class Op, int OUT, int NT, int CH>
+template <class Op, int OUT, int NT, int CH, bool ADD>
 __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(LinearArgs a, int64_t tiles) {
     constexpr int P = 2;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -254,7 +251,14 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
     }
     __syncthreads();
 
+    // what the work on a tile's sums reads of its rows: requested with them, not when it is needed (that
+    // wait would also be one for the next tile's rows)
+    struct Side {
+        float xs;
+        unsigned bits[NT];
+    };
     typename Op::Raw raw[CH][P];
+    Side next[P];
     auto row_of = [&](int64_t tile, int j) {
         const int64_t p = tile * (16 * P) + 16 * j + r;
         return p < a.n ? p : a.n - 1;  // a lane behind the last row repeats it and stores nothing
@@ -263,6 +267,15 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
 #pragma unroll
         for (int j = 0; j < P; ++j) {
             const int64_t p = row_of(tile, j);
+            if (s0 == 0) {
+                if constexpr (Op::kInt8) {
+                    next[j].xs = a.scale[p];
+                } else {
+#pragma unroll
+                    for (int T = 0; T < NT; ++T)
+                        next[j].bits[T] = T0 + T < a.groups ? mask_bits(a, p, 64 * (T0 + T) + 16 * g) : 0u;
+                }
+            }
 #pragma unroll
             for (int i = 0; i < CH; ++i)
                 if (s0 + i < a.steps) raw[i][j] = Op::fetch(a, p, s0 + i, g);
@@ -297,6 +310,9 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
                 }
             }
         }
+        Side now[P];
+#pragma unroll
+        for (int j = 0; j < P; ++j) now[j] = next[j];
         if (tile + stride < tiles) fetch(tile + stride, 0);
 #pragma unroll
         for (int j = 0; j < P; ++j) {
@@ -305,27 +321,32 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
             if constexpr (!Op::kInt8) {
                 if (live) {
 #pragma unroll
-                    for (int T = 0; T < NT; ++T) put_grad<OUT>(a, acc[j][T], 64 * (T0 + T) + 16 * g, p);
+                    for (int T = 0; T < NT; ++T) {
+                        if (T0 + T < a.groups)
+                            put_grad<OUT>(a, acc[j][T], 64 * (T0 + T) + 16 * g, p, 64 * (T0 + T) + 64 <= a.features, now[j].bits[T]);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
                 }
             } else if constexpr (OUT != TO_INT8) {
-                const float xs = a.scale[p];
 #pragma unroll
                 for (int T = 0; T < NT; ++T) {
                     const int f = 64 * (T0 + T) + 16 * g;
-                    if (live && f < a.features) {
+                    const bool whole = 64 * (T0 + T) + 64 <= a.features;
+                    if (T0 + T < a.groups && live) {
                         float v[16];
-                        finish_linear(a, acc[j][T], ws + 64 * T + 16 * g, bs + 64 * T + 16 * g, xs, f, p, v);
-                        store16<OUT>(a, p, f, v);
+                        finish_linear<ADD>(a, acc[j][T], ws + 64 * T + 16 * g, bs + 64 * T + 16 * g, now[j].xs, f, p, whole, v);
+                        put<OUT>(a, p, f, whole, v);
                     }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             } else {
                 // the whole row is here (16 features per group in each of 4 lanes): its scale, then its integers
-                const float xs = a.scale[p];
                 float v[NT][16];
                 unsigned top = 0u;
 #pragma unroll
                 for (int T = 0; T < NT; ++T) {
-                    finish_linear(a, acc[j][T], ws + 64 * T + 16 * g, bs + 64 * T + 16 * g, xs, 64 * T + 16 * g, p, v[T]);
+                    finish_linear<ADD>(a, acc[j][T], ws + 64 * T + 16 * g, bs + 64 * T + 16 * g, now[j].xs, 64 * T + 16 * g, p,
+                                       64 * T + 64 <= a.features, v[T]);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const unsigned m = magnitude(v[T][i]);
@@ -348,13 +369,13 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
                             unsigned o[4], bits = 0u;
 #pragma unroll
                             for (int w = 0; w < 4; ++w) {
-                                int t[4];
+                                float t[4];
 #pragma unroll
                                 for (int b = 0; b < 4; ++b) {
-                                    t[b] = quantised(v[T][4 * w + b], sc.inv);
+                                    t[b] = v[T][4 * w + b] * sc.inv;
                                     bits |= v[T][4 * w + b] > 0.f ? 1u << (4 * w + b) : 0u;
                                 }
-                                o[w] = pack4(t[0], t[1], t[2], t[3]);
+                                o[w] = sc.inv == 0.f ? 0u : round4(t);
                             }
                             *(uint4*)((signed char*)a.out + p * fp + 64 * T + 16 * g) = make_uint4(o[0], o[1], o[2], o[3]);
                             if (a.out_mask) *(unsigned short*)(a.out_mask + p * (fp / 8) + 8 * T + 2 * g) = (unsigned short)bits;
@@ -369,10 +390,10 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
 
 constexpr int kLdsBytes = 160 * 1024;
 
-template <class Op, int OUT, int NT, int CH>
+template <class Op, int OUT, int NT, int CH, bool ADD>
 int launch_resident(const LinearArgs& a, const char* what, hipStream_t st) {
     const size_t lds = channel_bytes<NT>() + (size_t)NT * a.steps * 4096;
-    auto kernel = linear_resident_kernel<Op, OUT, NT, CH>;
+    auto kernel = linear_resident_kernel<Op, OUT, NT, CH, ADD>;
     // (the limit is an attribute of the function on every device; asking again costs nothing)
     const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes);
     if (e != hipSuccess) return NERF_FAIL((int)e, "%s: %s", what, hipGetErrorString(e));
@@ -387,11 +408,11 @@ int launch_resident(const LinearArgs& a, const char* what, hipStream_t st) {
     return check_launch(what);
 }
 
-template <class Op, int DT>
+template <class Op, int DT, bool ADD>
 int launch_direct(const LinearArgs& a, const char* what, hipStream_t st) {
     const int64_t waves = (a.n + 31) / 32 * a.groups;
     if ((waves + 3) / 4 >= (1LL << 24)) return NERF_FAIL(NERF_E_UNSUPPORTED, "%s: too many rows", what);
-    linear_direct_kernel<Op, DT><<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(a);
+    linear_direct_kernel<Op, DT, ADD><<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(a);
     return check_launch(what);
 }
 

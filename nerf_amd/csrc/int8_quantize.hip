@@ -44,13 +44,13 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const void* __restri
         signed char* qr = q + row * kp;
         unsigned char* mr = mask ? mask + row * (kp / 8) : nullptr;
         auto write = [&](int c, const float (&w)[8]) {
-            int t[8];
+            float lo[4], hi[4];
             unsigned bits = 0u;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) t[i] = quantised(w[i], sc.inv), bits |= w[i] > 0.f ? 1u << i : 0u;
-            uint2 o;
-            o.x = pack4(t[0], t[1], t[2], t[3]), o.y = pack4(t[4], t[5], t[6], t[7]);
-            *(uint2*)(qr + 8 * c) = o;
+            for (int i = 0; i < 4; ++i) lo[i] = w[i] * sc.inv, hi[i] = w[i + 4] * sc.inv;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) bits |= w[i] > 0.f ? 1u << i : 0u;
+            *(uint2*)(qr + 8 * c) = sc.inv == 0.f ? make_uint2(0u, 0u) : make_uint2(round4(lo), round4(hi));
             if (mr) mr[c] = (unsigned char)bits;
         };
         if constexpr (NV > 0) {
