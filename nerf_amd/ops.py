@@ -422,10 +422,29 @@ def _on_gpu(what, *tensors):
             raise ValueError(f"{what}: expected tensors, got {type(t).__name__}")
         if not t.is_cuda:
             raise nv.NerfHipError(f"{what}: expected a tensor on the GPU (the HIP path has no CPU fallback)")
-        if dev is not None and t.device != dev:
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
             raise ValueError(f"{what}: tensors on {dev} and {t.device}")
-        dev = t.device
     return dev
+
+
+def _call(name, dev, *args):
+    """One entry point on `dev` and its current stream; device pointers as integers.  (A call for one ray is
+    all host time: no context manager and no stream object where the device is the current one.)"""
+    fn = getattr(nv.lib(), name)
+    index = dev.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        nv.check(rc, name)
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _row_major(what, t, width=None):
@@ -461,6 +480,13 @@ class Int8Rows:
             raise ValueError("Int8Rows: expected contiguous tensors")
         self.q, self.scale, self.k, self.pow2, self.mask = q, scale, k, bool(pow2), mask
 
+    @classmethod
+    def _made(cls, q, scale, k, pow2, mask):
+        """Of tensors that _new_rows made."""
+        self = cls.__new__(cls)
+        self.q, self.scale, self.k, self.pow2, self.mask = q, scale, k, bool(pow2), mask
+        return self
+
     @property
     def n(self):
         return self.q.shape[0]
@@ -494,10 +520,9 @@ def quantize_rows(x, pow2=False, want_mask=False):
     x, ld = _row_major("quantize_rows", x)
     n, k = x.shape
     q, scale, mask = _new_rows(n, k, dev, want_mask)
-    with torch.cuda.device(dev):
-        nv.check(nv.lib().nerf_quantize_rows(ctypes.c_void_p(x.data_ptr()), _DTYPES[x.dtype], n, k, ld, int(bool(pow2)),
-                                             nv.ptr(q), nv.ptr(scale), nv.ptr(mask), nv.stream()), "nerf_quantize_rows")
-    return Int8Rows(q, scale, k, pow2, mask)
+    _call("nerf_quantize_rows", dev, x.data_ptr(), _DTYPES[x.dtype], n, k, ld, 1 if pow2 else 0, q.data_ptr(), scale.data_ptr(),
+          _addr(mask))
+    return Int8Rows._made(q, scale, k, pow2, mask)
 
 
 def pack_int8(w, pow2=False):
@@ -512,8 +537,7 @@ def pack_int8(w, pow2=False):
     if need == 0:
         raise ValueError(f"pack_int8: widths {k} x {m} are beyond what the kernels are built for")
     packed = torch.empty((need,), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        nv.check(nv.lib().nerf_int8_pack(nv.ptr(w), k, m, int(bool(pow2)), nv.ptr(packed), nv.stream()), "nerf_int8_pack")
+    _call("nerf_int8_pack", dev, w.data_ptr(), k, m, 1 if pow2 else 0, packed.data_ptr())
     return Int8Weights(packed, k, m, bool(pow2))
 
 
@@ -524,7 +548,8 @@ def _linear_inputs(what, rows, weights, bias, addend):
     if rows.k != weights.k:
         raise ValueError(f"{what}: rows of {rows.k} elements against weights for {weights.k}")
     if bias is not None:
-        bias = nv.f32(bias.detach(), dev)
+        if bias.dtype != torch.float32 or not bias.is_contiguous():
+            bias = nv.f32(bias.detach(), dev)
         if tuple(bias.shape) != (weights.m,):
             raise ValueError(f"{what}: bias must be [{weights.m}], got {tuple(bias.shape)}")
     ldadd, add_dtype = 0, 0
@@ -542,12 +567,10 @@ def linear_int8(rows, weights, bias=None, relu=False, addend=None, dtype=torch.f
     dev, bias, addend, add_dtype, ldadd = _linear_inputs("linear_int8", rows, weights, bias, addend)
     if dtype not in _DTYPES:
         raise ValueError(f"linear_int8: dtype must be float32, float16 or bfloat16, got {dtype}")
-    y = torch.empty((rows.n, weights.m), dtype=dtype, device=dev)
-    with torch.cuda.device(dev):
-        nv.check(nv.lib().nerf_linear_int8(nv.ptr(rows.q), nv.ptr(rows.scale), rows.n, rows.k, nv.ptr(weights.packed),
-                                           weights.m, nv.ptr(bias), None if addend is None else ctypes.c_void_p(addend.data_ptr()),
-                                           add_dtype, ldadd, int(bool(relu)), nv.ptr(y), _DTYPES[dtype], weights.m,
-                                           nv.stream()), "nerf_linear_int8")
+    n, m = rows.n, weights.m
+    y = torch.empty((n, m), dtype=dtype, device=dev)
+    _call("nerf_linear_int8", dev, rows.q.data_ptr(), rows.scale.data_ptr(), n, rows.k, weights.packed.data_ptr(), m, _addr(bias),
+          _addr(addend), add_dtype, ldadd, 1 if relu else 0, y.data_ptr(), _DTYPES[dtype], m)
     return y
 
 
@@ -557,14 +580,11 @@ def linear_int8_quantized(rows, weights, bias=None, relu=False, addend=None, pow
     dev, bias, addend, add_dtype, ldadd = _linear_inputs("linear_int8_quantized", rows, weights, bias, addend)
     if weights.m > nv.lib().nerf_linear_int8_quantized_width(rows.k):
         return quantize_rows(linear_int8(rows, weights, bias, relu, addend), pow2, want_mask)
-    q, scale, mask = _new_rows(rows.n, weights.m, dev, want_mask)
-    with torch.cuda.device(dev):
-        nv.check(nv.lib().nerf_linear_int8_quantized(nv.ptr(rows.q), nv.ptr(rows.scale), rows.n, rows.k, nv.ptr(weights.packed),
-                                                     weights.m, nv.ptr(bias),
-                                                     None if addend is None else ctypes.c_void_p(addend.data_ptr()), add_dtype,
-                                                     ldadd, int(bool(relu)), int(bool(pow2)), nv.ptr(q), nv.ptr(scale),
-                                                     nv.ptr(mask), nv.stream()), "nerf_linear_int8_quantized")
-    return Int8Rows(q, scale, weights.m, pow2, mask)
+    n, m = rows.n, weights.m
+    q, scale, mask = _new_rows(n, m, dev, want_mask)
+    _call("nerf_linear_int8_quantized", dev, rows.q.data_ptr(), rows.scale.data_ptr(), n, rows.k, weights.packed.data_ptr(), m,
+          _addr(bias), _addr(addend), add_dtype, ldadd, 1 if relu else 0, 1 if pow2 else 0, q.data_ptr(), scale.data_ptr(), _addr(mask))
+    return Int8Rows._made(q, scale, m, pow2, mask)
 
 
 def linear_int8_grad_input(dz, weights, mask=None):
@@ -578,13 +598,13 @@ def linear_int8_grad_input(dz, weights, mask=None):
     dev = _on_gpu(what, dz, weights.packed, mask)
     dz, ld = _row_major(what, dz, weights.m)
     n = dz.shape[0]
+    if mask is not None and not mask.is_contiguous():
+        mask = mask.contiguous()
     if mask is not None and (mask.dtype != torch.uint8 or tuple(mask.shape) != (n, _padded_width(weights.k) // 8)):
         raise ValueError(f"{what}: mask must be uint8 [{n}, {_padded_width(weights.k) // 8}], got {mask.dtype} {tuple(mask.shape)}")
     dx = torch.empty((n, weights.k), dtype=dz.dtype, device=dev)
-    with torch.cuda.device(dev):
-        nv.check(nv.lib().nerf_linear_int8_grad_input(ctypes.c_void_p(dz.data_ptr()), _DTYPES[dz.dtype], n, weights.m, ld,
-                                                      nv.ptr(weights.packed), weights.k, nv.ptr(mask), nv.ptr(dx), weights.k,
-                                                      nv.stream()), "nerf_linear_int8_grad_input")
+    _call("nerf_linear_int8_grad_input", dev, dz.data_ptr(), _DTYPES[dz.dtype], n, weights.m, ld, weights.packed.data_ptr(), weights.k,
+          _addr(mask), dx.data_ptr(), weights.k)
     return dx
 
 
@@ -607,9 +627,6 @@ def linear_int8_grad_weight(rows, dz):
     db = torch.empty((m,), dtype=torch.float32, device=dev)
     need = int(nv.lib().nerf_linear_int8_grad_weight_bytes(n, rows.k, m))
     ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
-    with torch.cuda.device(dev):
-        nv.check(nv.lib().nerf_linear_int8_grad_weight(nv.ptr(rows.q), nv.ptr(rows.scale), n, rows.k,
-                                                       ctypes.c_void_p(dz.data_ptr()), _DTYPES[dz.dtype], m, ld, nv.ptr(dw),
-                                                       nv.ptr(db), nv.ptr(ws), need, nv.stream()),
-                 "nerf_linear_int8_grad_weight")
+    _call("nerf_linear_int8_grad_weight", dev, rows.q.data_ptr(), rows.scale.data_ptr(), n, rows.k, dz.data_ptr(), _DTYPES[dz.dtype], m,
+          ld, dw.data_ptr(), db.data_ptr(), _addr(ws), need)
     return dw, db
