@@ -6,8 +6,8 @@ namespace i8 {
 
 constexpr int64_t kResidentRows = 4096;
 
-// Steps of dz rows held in registers: all of 256 columns where they fit beside the sums.
-template <int DT> constexpr int kHeld = DT == NERF_BF16 ? 8 : DT == NERF_F16 ? 4 : 3;
+// Steps of dz rows in a unit: 256 columns of 16-bit types, 128 of fp32 (32 registers).
+template <int DT> constexpr int kHeld = DT == NERF_F32 ? 4 : 8;
 
 template <int DT, int NT>
 static int resident(const LinearArgs& a, const char* what, hipStream_t st) {

@@ -9,8 +9,13 @@ constexpr int64_t kResidentRows = 4096;
 
 template <int OUT, int NT, bool ADD>
 static int resident(const LinearArgs& a, const char* what, hipStream_t st) {
-    if (a.steps <= 2) return launch_resident<Int8Op, OUT, NT, 2, ADD>(a, what, st);
-    return launch_resident<Int8Op, OUT, NT, 5, ADD>(a, what, st);
+    switch (a.steps) {  // all of a row in one unit up to 320 inputs
+        case 1: return launch_resident<Int8Op, OUT, NT, 1, ADD>(a, what, st);
+        case 2: return launch_resident<Int8Op, OUT, NT, 2, ADD>(a, what, st);
+        case 5: return launch_resident<Int8Op, OUT, NT, 5, ADD>(a, what, st);
+        case 3: case 6: case 9: return launch_resident<Int8Op, OUT, NT, 3, ADD>(a, what, st);
+        default: return launch_resident<Int8Op, OUT, NT, 4, ADD>(a, what, st);
+    }
 }
 
 template <int OUT, bool ADD>

@@ -220,17 +220,19 @@ __global__ __launch_bounds__(256) void linear_direct_kernel(LinearArgs a) {
 }
 
 // Many rows, weights that fit LDS: a workgroup per CU copies the fragments of up to NT groups of
-// features into LDS once and its eight waves then stream tiles of 32 points past them.  A wave holds
-// the sums of all NT groups of a tile (64 NT registers of 32), so a row is read once; the next tile's
-// rows are requested as soon as the last product has read the registers they go to, and arrive
-// behind the work on the sums.  CH steps of rows are held at a time.
-constexpr int kResidentThreads = 512;
+// features into LDS once and its eight waves then stream tiles of 16 points past them.  A wave holds
+// the sums of all NT groups of a tile (16 NT registers), so a row is read once, and its work is a run of
+// units: CH steps of a tile's rows.  While one unit is worked on, the next one's rows (of this tile or the
+// next) are on their way into the other half of the registers, so that loads are in flight all the
+// time; tiles of 32 points, which halve the reads of LDS, leave no room for that (786432 x 256 x 256,
+// input gradient: 249 us).  A fetch is the same loads on every path (a step behind the last repeats it,
+// a tile behind the last repeats the one at hand): a wait for older loads counts the younger ones.
+constexpr int kResidentThreads = 512, kTile = 16;
 template <int NT>
 constexpr int channel_bytes() { return 2 * NT * 64 * 4; }
 
 template <class Op, int OUT, int NT, int CH, bool ADD>
 __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(LinearArgs a, int64_t tiles) {
-    constexpr int P = 2;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float* const ws = (float*)lds;
     float* const bs = ws + NT * 64;
@@ -252,138 +254,141 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
     __syncthreads();
 
     // what the work on a tile's sums reads of its rows: requested with them, not when it is needed (that
-    // wait would also be one for the next tile's rows)
+    // wait would also be one for the next unit's rows)
     struct Side {
         float xs;
         unsigned bits[NT];
     };
-    typename Op::Raw raw[CH][P];
-    Side next[P];
-    auto row_of = [&](int64_t tile, int j) {
-        const int64_t p = tile * (16 * P) + 16 * j + r;
+    typename Op::Raw raw[2][CH];
+    Side side[2];  // of the tile being worked on, of the one being fetched
+    typename Op::Acc acc[NT][4];
+    auto row_of = [&](int64_t tile) {
+        const int64_t p = tile * kTile + r;
         return p < a.n ? p : a.n - 1;  // a lane behind the last row repeats it and stores nothing
     };
-    auto fetch = [&](int64_t tile, int s0) {
+    // bits of the mask: without one, any bytes, all set afterwards
+    const unsigned char* const mask = a.mask ? a.mask : (const unsigned char*)a.frags;
+    const int64_t mask_ld = a.mask ? a.groups * 8 : 0;
+    const unsigned no_mask = a.mask ? 0u : 0xffffu;
+    auto fetch = [&](int64_t tile, int s0, typename Op::Raw (&to)[CH]) {
+        const int64_t p = row_of(tile);
+        if constexpr (Op::kInt8) {
+            side[1].xs = a.scale[p];
+        } else {
 #pragma unroll
-        for (int j = 0; j < P; ++j) {
-            const int64_t p = row_of(tile, j);
-            if (s0 == 0) {
-                if constexpr (Op::kInt8) {
-                    next[j].xs = a.scale[p];
-                } else {
-#pragma unroll
-                    for (int T = 0; T < NT; ++T)
-                        next[j].bits[T] = T0 + T < a.groups ? mask_bits(a, p, 64 * (T0 + T) + 16 * g) : 0u;
-                }
+            for (int T = 0; T < NT; ++T) {
+                const int t = T0 + T < a.groups ? T0 + T : a.groups - 1;
+                side[1].bits[T] = *(const unsigned short*)(mask + p * mask_ld + 8 * t + 2 * g) | no_mask;
             }
+        }
 #pragma unroll
-            for (int i = 0; i < CH; ++i)
-                if (s0 + i < a.steps) raw[i][j] = Op::fetch(a, p, s0 + i, g);
+        for (int i = 0; i < CH; ++i) to[i] = Op::fetch(a, p, s0 + i < a.steps ? s0 + i : a.steps - 1, g);
+    };
+    auto multiply = [&](int s0, const typename Op::Raw (&from)[CH]) {
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            if (s0 + i < a.steps) {
+                const char* w = wl + (s0 + i) * (NT * 4096) + lane * 16;
+                const typename Op::B b(from[i]);
+#pragma unroll
+                for (int T = 0; T < NT; ++T)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) acc[T][u] = Op::mma(*(const i32x4*)(w + (T * 4 + u) * 1024), b, acc[T][u]);
+            }
         }
     };
-    const int64_t stride = (int64_t)gridDim.x * (kResidentThreads / 64);
-    int64_t tile = (int64_t)blockIdx.x * (kResidentThreads / 64) + wave;
-    if (tile < tiles) fetch(tile, 0);
-    for (; tile < tiles; tile += stride) {
-        typename Op::Acc acc[P][NT][4];
+    auto finish = [&](int64_t tile) {
+        const int64_t p = row_of(tile);
+        const bool live = tile * kTile + r < a.n;
+        const Side& now = side[0];
+        if constexpr (!Op::kInt8) {
+            if (live) {
 #pragma unroll
-        for (int j = 0; j < P; ++j)
+                for (int T = 0; T < NT; ++T) {
+                    if (T0 + T < a.groups)
+                        put_grad<OUT>(a, acc[T], 64 * (T0 + T) + 16 * g, p, 64 * (T0 + T) + 64 <= a.features, now.bits[T]);
+                }
+            }
+        } else if constexpr (OUT != TO_INT8) {
 #pragma unroll
-            for (int T = 0; T < NT; ++T)
+            for (int T = 0; T < NT; ++T) {
+                const int f = 64 * (T0 + T) + 16 * g;
+                const bool whole = 64 * (T0 + T) + 64 <= a.features;
+                if (T0 + T < a.groups && live) {
+                    float v[16];
+                    finish_linear<ADD>(a, acc[T], ws + 64 * T + 16 * g, bs + 64 * T + 16 * g, now.xs, f, p, whole, v);
+                    put<OUT>(a, p, f, whole, v);
+                }
+            }
+        } else {
+            // the whole row is here (16 features per group in each of 4 lanes): its scale, then its integers
+            float v[NT][16];
+            unsigned top = 0u;
 #pragma unroll
-                for (int u = 0; u < 4; ++u) acc[j][T][u] = typename Op::Acc{};
-        for (int s0 = 0; s0 < a.steps; s0 += CH) {
-            if (s0) fetch(tile, s0);
+            for (int T = 0; T < NT; ++T) {
+                finish_linear<ADD>(a, acc[T], ws + 64 * T + 16 * g, bs + 64 * T + 16 * g, now.xs, 64 * T + 16 * g, p,
+                                   64 * T + 64 <= a.features, v[T]);
 #pragma unroll
-            for (int i = 0; i < CH; ++i) {
-                if (s0 + i < a.steps) {
-                    const char* w = wl + (s0 + i) * (NT * 4096) + lane * 16;
-                    const typename Op::B b0(raw[i][0]), b1(raw[i][1]);
+                for (int i = 0; i < 16; ++i) {
+                    const unsigned m = magnitude(v[T][i]);
+                    top = top > m ? top : m;
+                }
+                __builtin_amdgcn_sched_barrier(0);  // in turn: 16 sums become 16 values in the same registers
+            }
 #pragma unroll
-                    for (int T = 0; T < NT; ++T)
+            for (int off = 16; off < 64; off *= 2) {
+                const unsigned o = (unsigned)__shfl_xor((int)top, off);
+                top = top > o ? top : o;
+            }
+            const Scale sc = scale_of(top, a.pow2 != 0);
+            const int fp = a.groups * 64;  // width of a row of the output
+            if (live) {
+                if (g == 0) a.out_scale[p] = sc.scale;
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            const i32x4 wf = *(const i32x4*)(w + (T * 4 + u) * 1024);
-                            acc[0][T][u] = Op::mma(wf, b0, acc[0][T][u]);
-                            acc[1][T][u] = Op::mma(wf, b1, acc[1][T][u]);
+                for (int T = 0; T < NT; ++T) {
+                    if (T < a.groups) {
+                        unsigned o[4], bits = 0u;
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            float t[4];
+#pragma unroll
+                            for (int b = 0; b < 4; ++b) {
+                                t[b] = v[T][4 * w + b] * sc.inv;
+                                bits |= v[T][4 * w + b] > 0.f ? 1u << (4 * w + b) : 0u;
+                            }
+                            o[w] = round4(t);
                         }
+                        if (sc.inv == 0.f) o[0] = o[1] = o[2] = o[3] = 0u;
+                        *(uint4*)((signed char*)a.out + p * fp + 64 * T + 16 * g) = make_uint4(o[0], o[1], o[2], o[3]);
+                        if (a.out_mask) *(unsigned short*)(a.out_mask + p * (fp / 8) + 8 * T + 2 * g) = (unsigned short)bits;
+                    }
                 }
             }
         }
-        Side now[P];
+    };
+
+    const int64_t stride = (int64_t)gridDim.x * (kResidentThreads / 64);
+    int64_t tile = (int64_t)blockIdx.x * (kResidentThreads / 64) + wave;
+    int s0 = 0;
+    if (tile < tiles) fetch(tile, 0, raw[0]);
+    while (tile < tiles) {
 #pragma unroll
-        for (int j = 0; j < P; ++j) now[j] = next[j];
-        if (tile + stride < tiles) fetch(tile + stride, 0);
+        for (int h = 0; h < 2; ++h) {
+            if (tile >= tiles) break;
+            const bool last = s0 + CH >= a.steps;
+            const int64_t tile1 = last ? tile + stride : tile;
+            const int s1 = last ? 0 : s0 + CH;
+            if (s0 == 0) {
+                side[0] = side[1];
 #pragma unroll
-        for (int j = 0; j < P; ++j) {
-            const int64_t p = row_of(tile, j);
-            const bool live = tile * (16 * P) + 16 * j + r < a.n;
-            if constexpr (!Op::kInt8) {
-                if (live) {
+                for (int T = 0; T < NT; ++T)
 #pragma unroll
-                    for (int T = 0; T < NT; ++T) {
-                        if (T0 + T < a.groups)
-                            put_grad<OUT>(a, acc[j][T], 64 * (T0 + T) + 16 * g, p, 64 * (T0 + T) + 64 <= a.features, now[j].bits[T]);
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-                }
-            } else if constexpr (OUT != TO_INT8) {
-#pragma unroll
-                for (int T = 0; T < NT; ++T) {
-                    const int f = 64 * (T0 + T) + 16 * g;
-                    const bool whole = 64 * (T0 + T) + 64 <= a.features;
-                    if (T0 + T < a.groups && live) {
-                        float v[16];
-                        finish_linear<ADD>(a, acc[j][T], ws + 64 * T + 16 * g, bs + 64 * T + 16 * g, now[j].xs, f, p, whole, v);
-                        put<OUT>(a, p, f, whole, v);
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-            } else {
-                // the whole row is here (16 features per group in each of 4 lanes): its scale, then its integers
-                float v[NT][16];
-                unsigned top = 0u;
-#pragma unroll
-                for (int T = 0; T < NT; ++T) {
-                    finish_linear<ADD>(a, acc[j][T], ws + 64 * T + 16 * g, bs + 64 * T + 16 * g, now[j].xs, 64 * T + 16 * g, p,
-                                       64 * T + 64 <= a.features, v[T]);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const unsigned m = magnitude(v[T][i]);
-                        top = top > m ? top : m;
-                    }
-                    __builtin_amdgcn_sched_barrier(0);  // in turn: 16 sums become 16 values in the same registers
-                }
-#pragma unroll
-                for (int off = 16; off < 64; off *= 2) {
-                    const unsigned o = (unsigned)__shfl_xor((int)top, off);
-                    top = top > o ? top : o;
-                }
-                const Scale sc = scale_of(top, a.pow2 != 0);
-                const int fp = a.groups * 64;  // width of a row of the output
-                if (live) {
-                    if (g == 0) a.out_scale[p] = sc.scale;
-#pragma unroll
-                    for (int T = 0; T < NT; ++T) {
-                        if (T < a.groups) {
-                            unsigned o[4], bits = 0u;
-#pragma unroll
-                            for (int w = 0; w < 4; ++w) {
-                                float t[4];
-#pragma unroll
-                                for (int b = 0; b < 4; ++b) {
-                                    t[b] = v[T][4 * w + b] * sc.inv;
-                                    bits |= v[T][4 * w + b] > 0.f ? 1u << (4 * w + b) : 0u;
-                                }
-                                o[w] = sc.inv == 0.f ? 0u : round4(t);
-                            }
-                            *(uint4*)((signed char*)a.out + p * fp + 64 * T + 16 * g) = make_uint4(o[0], o[1], o[2], o[3]);
-                            if (a.out_mask) *(unsigned short*)(a.out_mask + p * (fp / 8) + 8 * T + 2 * g) = (unsigned short)bits;
-                        }
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-                }
+                    for (int u = 0; u < 4; ++u) acc[T][u] = typename Op::Acc{};
             }
+            fetch(tile1 < tiles ? tile1 : tile, s1, raw[h ^ 1]);
+            multiply(s0, raw[h]);
+            if (last) finish(tile);
+            tile = tile1, s0 = s1;
         }
     }
 }
@@ -399,7 +404,7 @@ int launch_resident(const LinearArgs& a, const char* what, hipStream_t st) {
     if (e != hipSuccess) return NERF_FAIL((int)e, "%s: %s", what, hipGetErrorString(e));
     int cus = device_cu_count();
     if (cus <= 0) cus = 256;
-    const int64_t tiles = (a.n + 31) / 32;
+    const int64_t tiles = (a.n + kTile - 1) / kTile;
     const int fblocks = (a.groups + NT - 1) / NT;
     int64_t blocks = (tiles + kResidentThreads / 64 - 1) / (kResidentThreads / 64);
     const int64_t most = cus / fblocks > 0 ? cus / fblocks : 1;
