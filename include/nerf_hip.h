@@ -313,8 +313,9 @@ size_t nerf_int8_packed_bytes(int k, int m, int pow2);
 int nerf_int8_pack(const float* w, int k, int m, int pow2, void* packed, nerf_stream_t stream);
 
 /* y [n][m] = ((sum_f q[i][f] p[f][j]) * channel scale j) * row scale i (+ bias[j]) (+ addend[i][j]), then
- * relu when asked; the integer sums are exact, every later step is rounded to fp32, the result to y's
- * type.  bias [m] or NULL; addend: [n][m] of any of the three types or NULL; y must not overlap an
+ * relu when asked; the integer sums are exact; in fp32 are rounded: the sum, its product with the
+ * channel scale, that times the row scale plus the bias (once), the addition of the addend; the result
+ * to y's type.  bias [m] or NULL; addend: [n][m] of any of the three types or NULL; y must not overlap an
  * input. */
 int nerf_linear_int8(const signed char* q, const float* scale, int64_t n, int k, const void* packed, int m,
                      const float* bias, const void* addend, int addend_dtype, int64_t ldadd, int relu,

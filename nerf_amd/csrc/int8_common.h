@@ -248,13 +248,14 @@ DEV unsigned pack4(int a, int b, int c, int d) {
     return (unsigned)(a & 255) | (unsigned)(b & 255) << 8 | (unsigned)(c & 255) << 16 | (unsigned)d << 24;
 }
 
-// Four finite numbers of magnitude at most 127.5 rounded to bytes, halves to even: added to 1.5 x 2^23, where
-// a float's step is 1, they leave the integer in its low byte (one addition instead of a rounding and
-// a conversion, and a byte permutation instead of masks and shifts).
-DEV unsigned round4(const float (&t)[4]) {
+// Rounding to bytes, halves to even: a number of magnitude at most 127.5 added to 1.5 x 2^23, where a
+// float's step is 1, leaves its integer in the low byte (one addition instead of a rounding and a
+// conversion); four low bytes are gathered with byte permutations.
+constexpr float kRoundAt = 12582912.f;
+DEV unsigned low_bytes(const float (&t)[4]) {
     unsigned b[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) b[i] = __builtin_bit_cast(unsigned, t[i] + 12582912.f);
+    for (int i = 0; i < 4; ++i) b[i] = __builtin_bit_cast(unsigned, t[i]);
     const unsigned lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u);
     return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
 }

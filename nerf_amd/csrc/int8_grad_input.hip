@@ -11,9 +11,9 @@ template <int DT> constexpr int kHeld = DT == NERF_F32 ? 4 : 8;
 
 template <int DT, int NT>
 static int resident(const LinearArgs& a, const char* what, hipStream_t st) {
-    if (a.width % 32 != 0) return launch_resident<Bf16Op<DT, false>, DT, NT, 2, false>(a, what, st);
-    if (a.steps <= 2) return launch_resident<Bf16Op<DT, true>, DT, NT, 2, false>(a, what, st);
-    return launch_resident<Bf16Op<DT, true>, DT, NT, kHeld<DT>, false>(a, what, st);
+    if (a.width % 32 != 0) return launch_resident<Bf16Op<DT, false>, DT, NT, 2, 1, false>(a, what, st);
+    if (a.steps <= 2) return launch_resident<Bf16Op<DT, true>, DT, NT, 2, 1, false>(a, what, st);
+    return launch_resident<Bf16Op<DT, true>, DT, NT, kHeld<DT>, 1, false>(a, what, st);
 }
 
 template <int DT>

@@ -7,21 +7,25 @@ namespace i8 {
 // Rows from which the resident kernel's copy of the weights into every CU pays.
 constexpr int64_t kResidentRows = 4096;
 
+// Tiles of 16 points a wave works on at a time: two halve the reads of LDS and of the channel scales, where
+// the registers hold the sums of both.
+template <int OUT, int NT, int CH, bool ADD> constexpr int kTiles = (NT == 4 && (CH > 4 || ADD || OUT >= TO_INT8)) || (NT == 2 && ADD && OUT >= TO_INT8) ? 1 : 2;
+
 template <int OUT, int NT, bool ADD>
 static int resident(const LinearArgs& a, const char* what, hipStream_t st) {
     switch (a.steps) {  // all of a row in one unit up to 320 inputs
-        case 1: return launch_resident<Int8Op, OUT, NT, 1, ADD>(a, what, st);
-        case 2: return launch_resident<Int8Op, OUT, NT, 2, ADD>(a, what, st);
-        case 5: return launch_resident<Int8Op, OUT, NT, 5, ADD>(a, what, st);
-        case 3: case 6: case 9: return launch_resident<Int8Op, OUT, NT, 3, ADD>(a, what, st);
-        default: return launch_resident<Int8Op, OUT, NT, 4, ADD>(a, what, st);
+        case 1: return launch_resident<Int8Op, OUT, NT, 1, kTiles<OUT, NT, 1, ADD>, ADD>(a, what, st);
+        case 2: return launch_resident<Int8Op, OUT, NT, 2, kTiles<OUT, NT, 2, ADD>, ADD>(a, what, st);
+        case 5: return launch_resident<Int8Op, OUT, NT, 5, kTiles<OUT, NT, 5, ADD>, ADD>(a, what, st);
+        case 3: case 6: case 9: return launch_resident<Int8Op, OUT, NT, 3, kTiles<OUT, NT, 3, ADD>, ADD>(a, what, st);
+        default: return launch_resident<Int8Op, OUT, NT, 4, kTiles<OUT, NT, 4, ADD>, ADD>(a, what, st);
     }
 }
 
 template <int OUT, bool ADD>
 static int launch(const LinearArgs& a, const char* what, hipStream_t st) {
     const int nt = resident_groups(a);
-    if constexpr (OUT != TO_INT8) {
+    if constexpr (OUT < TO_INT8) {
         if (a.n < kResidentRows || nt == 0) return launch_direct<Int8Op, OUT, ADD>(a, what, st);
     }
     if (nt == 4) return resident<OUT, 4, ADD>(a, what, st);
@@ -90,6 +94,8 @@ NERF_API int nerf_linear_int8_quantized(const signed char* q, const float* scale
     if (n == 0) return 0;
     NERF_REQUIRE(yq && yscale, "%s: null pointer", what);
     NERF_REQUIRE(((uintptr_t)yq & 15) == 0 && ((uintptr_t)yscale & 3) == 0 && ((uintptr_t)ymask & 1) == 0, "%s: misaligned pointer", what);
-    a.out = yq, a.out_scale = yscale, a.out_mask = ymask, a.pow2 = pow2;
-    return launch<TO_INT8>(a, what, as_stream(stream));
+    a.out = yq, a.out_scale = yscale, a.out_mask = ymask;
+    hipStream_t st = as_stream(stream);
+    if (pow2) return relu ? launch<TO_INT8 + 3>(a, what, st) : launch<TO_INT8 + 2>(a, what, st);
+    return relu ? launch<TO_INT8 + 1>(a, what, st) : launch<TO_INT8>(a, what, st);
 }

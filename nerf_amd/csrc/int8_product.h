@@ -35,11 +35,11 @@ struct LinearArgs {
     // output in 8 bits (TO_INT8): out = integers, and
     float* out_scale;
     unsigned char* out_mask;
-    int pow2;
 };
 
-// What a product is stored as: a type (NERF_F32, ...) or 8-bit rows.
-constexpr int TO_INT8 = 3;
+// What a product is stored as: a type (NERF_F32, ...) or 8-bit rows: TO_INT8, + 1 behind a ReLU, + 2 with
+// scales that are powers of two.
+constexpr int TO_INT8 = 4;
 
 // ---- the two products -----------------------------------------------------------------------------
 // Raw: what a lane loads of a point's row for one step; B: the operands made of it.
@@ -103,16 +103,17 @@ DEV void add16(const T* row, int f, int width, bool whole, float (&v)[16]) {
 // A NaN with its sign bit clear, which the integer form of relu keeps; anything else as it is.
 DEV float positive_nan(float v) { return v != v ? __builtin_bit_cast(float, 0x7fc00000u) : v; }
 
-// y = relu((sum x channel scale) x row scale + bias + addend), each step rounded to fp32.  ws, b: the 16
-// channels' scales and biases (0 and 0 behind the last channel; a NaN without its sign).
+// y = relu((sum x channel scale) x row scale + bias + addend): the sum rounded to fp32, its product with
+// the channel scale rounded, then one rounding for row scale and bias and one for the addend.  ws, b: the
+// 16 channels' scales and biases (0 and 0 behind the last channel; a NaN without its sign).
 template <bool ADD>
 DEV void finish_linear(const LinearArgs& a, const i32x4 (&acc)[4], const float* ws, const float* b, float xs, int f, int64_t p,
-                       bool whole, float (&v)[16]) {
+                       bool whole, bool relu, float (&v)[16]) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
         const f32x4 w4 = *(const f32x4*)(ws + 4 * u), b4 = *(const f32x4*)(b + 4 * u);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[4 * u + r] = ((float)acc[u][r] * w4[r]) * xs + b4[r];
+        for (int r = 0; r < 4; ++r) v[4 * u + r] = __builtin_fmaf((float)acc[u][r] * w4[r], xs, b4[r]);
     }
     if constexpr (ADD) {
         if (a.add_dtype == NERF_F32) add16((const float*)a.addend + p * a.ldadd, f, a.features, whole, v);
@@ -121,13 +122,45 @@ DEV void finish_linear(const LinearArgs& a, const i32x4 (&acc)[4], const float* 
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = positive_nan(v[i]);
     }
-    if (a.relu) {  // a negative float is a negative integer: one instruction, and a NaN stays one
+    if (relu) {  // a negative float is a negative integer: one instruction, and a NaN stays one
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const int bits = __builtin_bit_cast(int, v[i]);
             v[i] = __builtin_bit_cast(float, bits > 0 ? bits : 0);
         }
     }
+}
+
+// One bit per value: v > 0.  Behind a ReLU (and without a NaN) that is a bit pattern other than zero, the
+// sign of its negative: a subtraction and a funnel shift a value (a comparison's result takes two wait
+// states to be read, and a selection to become a bit).
+template <bool RELU>
+DEV unsigned positive_bits(const float (&v)[16], bool has_nan) {
+    unsigned bits = 0u;
+    if (RELU && __builtin_expect(!has_nan, 1)) {
+#pragma unroll
+        for (int i = 15; i >= 0; --i) bits = __builtin_amdgcn_alignbit(bits, 0u - __builtin_bit_cast(unsigned, v[i]), 31);
+    } else {
+        if constexpr (RELU) asm volatile("");  // a branch that is hardly ever taken, not a selection between both
+#pragma unroll
+        for (int i = 0; i < 16; ++i) bits |= v[i] > 0.f ? 1u << i : 0u;
+    }
+    return bits;
+}
+
+// 16 values in bytes.  POW2: the product is exact, so the addition may take it in unrounded.
+template <bool POW2>
+DEV uint4 round16(const float (&v)[16], float inv) {
+    unsigned o[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        float t[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+            t[b] = POW2 ? __builtin_fmaf(v[4 * w + b], inv, kRoundAt) : v[4 * w + b] * inv + kRoundAt;
+        o[w] = low_bytes(t);
+    }
+    return inv == 0.f ? make_uint4(0u, 0u, 0u, 0u) : make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 template <int DT>
@@ -209,7 +242,7 @@ __global__ __launch_bounds__(256) void linear_direct_kernel(LinearArgs a) {
 #pragma unroll
         for (int j = 0; j < P; ++j) {
             float v[16];
-            finish_linear<ADD>(a, acc[j], &ch[wave][0][16 * g], &ch[wave][1][16 * g], a.scale[row[j]], f, row[j], whole, v);
+            finish_linear<ADD>(a, acc[j], &ch[wave][0][16 * g], &ch[wave][1][16 * g], a.scale[row[j]], f, row[j], whole, a.relu != 0, v);
             if (p0 + 16 * j + r < a.n) put<DT>(a, row[j], f, whole, v);
         }
     } else {
@@ -220,18 +253,18 @@ __global__ __launch_bounds__(256) void linear_direct_kernel(LinearArgs a) {
 }
 
 // Many rows, weights that fit LDS: a workgroup per CU copies the fragments of up to NT groups of
-// features into LDS once and its eight waves then stream tiles of 16 points past them.  A wave holds
-// the sums of all NT groups of a tile (16 NT registers), so a row is read once, and its work is a run of
+// features into LDS once and its eight waves then stream tiles of 16 P points past them.  A wave holds
+// the sums of all NT groups of a tile (16 NT P registers), so a row is read once, and its work is a run of
 // units: CH steps of a tile's rows.  While one unit is worked on, the next one's rows (of this tile or the
 // next) are on their way into the other half of the registers, so that loads are in flight all the
-// time; tiles of 32 points, which halve the reads of LDS, leave no room for that (786432 x 256 x 256,
-// input gradient: 249 us).  A fetch is the same loads on every path (a step behind the last repeats it,
+// time; with bf16 rows, tiles of 32 points, which halve the reads of LDS, leave no room for that (786432 x 256 x 256,
+// input gradient: 249 us; 8-bit rows are small enough for two tiles of 16 and both halves).  A fetch is the same loads on every path (a step behind the last repeats it,
 // a tile behind the last repeats the one at hand): a wait for older loads counts the younger ones.
-constexpr int kResidentThreads = 512, kTile = 16;
+constexpr int kResidentThreads = 512;
 template <int NT>
 constexpr int channel_bytes() { return 2 * NT * 64 * 4; }
 
-template <class Op, int OUT, int NT, int CH, bool ADD>
+template <class Op, int OUT, int NT, int CH, int P, bool ADD>
 __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(LinearArgs a, int64_t tiles) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float* const ws = (float*)lds;
@@ -259,109 +292,121 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
         float xs;
         unsigned bits[NT];
     };
-    typename Op::Raw raw[2][CH];
-    Side side[2];  // of the tile being worked on, of the one being fetched
-    typename Op::Acc acc[NT][4];
-    auto row_of = [&](int64_t tile) {
-        const int64_t p = tile * kTile + r;
+    typename Op::Raw raw[2][CH][P];
+    Side side[2][P];  // of the tile being worked on, of the one being fetched
+    typename Op::Acc acc[P][NT][4];
+    auto row_of = [&](int64_t tile, int j) {
+        const int64_t p = tile * (16 * P) + 16 * j + r;
         return p < a.n ? p : a.n - 1;  // a lane behind the last row repeats it and stores nothing
     };
     // bits of the mask: without one, any bytes, all set afterwards
     const unsigned char* const mask = a.mask ? a.mask : (const unsigned char*)a.frags;
     const int64_t mask_ld = a.mask ? a.groups * 8 : 0;
     const unsigned no_mask = a.mask ? 0u : 0xffffu;
-    auto fetch = [&](int64_t tile, int s0, typename Op::Raw (&to)[CH]) {
-        const int64_t p = row_of(tile);
-        if constexpr (Op::kInt8) {
-            side[1].xs = a.scale[p];
-        } else {
+    auto fetch = [&](int64_t tile, int s0, typename Op::Raw (&to)[CH][P]) {
 #pragma unroll
-            for (int T = 0; T < NT; ++T) {
-                const int t = T0 + T < a.groups ? T0 + T : a.groups - 1;
-                side[1].bits[T] = *(const unsigned short*)(mask + p * mask_ld + 8 * t + 2 * g) | no_mask;
+        for (int j = 0; j < P; ++j) {
+            const int64_t p = row_of(tile, j);
+            if constexpr (Op::kInt8) {
+                side[1][j].xs = a.scale[p];
+            } else {
+#pragma unroll
+                for (int T = 0; T < NT; ++T) {
+                    const int t = T0 + T < a.groups ? T0 + T : a.groups - 1;
+                    side[1][j].bits[T] = *(const unsigned short*)(mask + p * mask_ld + 8 * t + 2 * g) | no_mask;
+                }
             }
-        }
 #pragma unroll
-        for (int i = 0; i < CH; ++i) to[i] = Op::fetch(a, p, s0 + i < a.steps ? s0 + i : a.steps - 1, g);
+            for (int i = 0; i < CH; ++i) to[i][j] = Op::fetch(a, p, s0 + i < a.steps ? s0 + i : a.steps - 1, g);
+        }
     };
-    auto multiply = [&](int s0, const typename Op::Raw (&from)[CH]) {
+    auto multiply = [&](int s0, const typename Op::Raw (&from)[CH][P]) {
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             if (s0 + i < a.steps) {
                 const char* w = wl + (s0 + i) * (NT * 4096) + lane * 16;
-                const typename Op::B b(from[i]);
+                if constexpr (P == 1) {
+                    const typename Op::B b(from[i][0]);
 #pragma unroll
-                for (int T = 0; T < NT; ++T)
+                    for (int T = 0; T < NT; ++T)
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) acc[T][u] = Op::mma(*(const i32x4*)(w + (T * 4 + u) * 1024), b, acc[T][u]);
+                        for (int u = 0; u < 4; ++u) acc[0][T][u] = Op::mma(*(const i32x4*)(w + (T * 4 + u) * 1024), b, acc[0][T][u]);
+                } else {
+                    const typename Op::B b0(from[i][0]), b1(from[i][1]);
+#pragma unroll
+                    for (int T = 0; T < NT; ++T)
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            const i32x4 wf = *(const i32x4*)(w + (T * 4 + u) * 1024);
+                            acc[0][T][u] = Op::mma(wf, b0, acc[0][T][u]);
+                            acc[1][T][u] = Op::mma(wf, b1, acc[1][T][u]);
+                        }
+                }
             }
         }
     };
     auto finish = [&](int64_t tile) {
-        const int64_t p = row_of(tile);
-        const bool live = tile * kTile + r < a.n;
-        const Side& now = side[0];
-        if constexpr (!Op::kInt8) {
-            if (live) {
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            const int64_t p = row_of(tile, j);
+            const bool live = tile * (16 * P) + 16 * j + r < a.n;
+            const Side& now = side[0][j];
+            if constexpr (!Op::kInt8) {
+                if (live) {
+#pragma unroll
+                    for (int T = 0; T < NT; ++T) {
+                        if (T0 + T < a.groups)
+                            put_grad<OUT>(a, acc[j][T], 64 * (T0 + T) + 16 * g, p, 64 * (T0 + T) + 64 <= a.features, now.bits[T]);
+                    }
+                }
+            } else if constexpr (OUT < TO_INT8) {
 #pragma unroll
                 for (int T = 0; T < NT; ++T) {
-                    if (T0 + T < a.groups)
-                        put_grad<OUT>(a, acc[T], 64 * (T0 + T) + 16 * g, p, 64 * (T0 + T) + 64 <= a.features, now.bits[T]);
+                    const int f = 64 * (T0 + T) + 16 * g;
+                    const bool whole = 64 * (T0 + T) + 64 <= a.features;
+                    if (T0 + T < a.groups && live) {
+                        float v[16];
+                        finish_linear<ADD>(a, acc[j][T], ws + 64 * T + 16 * g, bs + 64 * T + 16 * g, now.xs, f, p, whole, a.relu != 0, v);
+                        put<OUT>(a, p, f, whole, v);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);  // in turn: 16 sums become 16 values in the same registers
                 }
-            }
-        } else if constexpr (OUT != TO_INT8) {
+            } else {
+                // the whole row is here (16 features per group in each of 4 lanes): its scale, then its integers
+                constexpr bool RELU = (OUT & 1) != 0, POW2 = (OUT & 2) != 0;
+                float v[NT][16];
+                unsigned top = 0u;
 #pragma unroll
-            for (int T = 0; T < NT; ++T) {
-                const int f = 64 * (T0 + T) + 16 * g;
-                const bool whole = 64 * (T0 + T) + 64 <= a.features;
-                if (T0 + T < a.groups && live) {
-                    float v[16];
-                    finish_linear<ADD>(a, acc[T], ws + 64 * T + 16 * g, bs + 64 * T + 16 * g, now.xs, f, p, whole, v);
-                    put<OUT>(a, p, f, whole, v);
+                for (int T = 0; T < NT; ++T) {
+                    finish_linear<ADD>(a, acc[j][T], ws + 64 * T + 16 * g, bs + 64 * T + 16 * g, now.xs, 64 * T + 16 * g, p,
+                                       64 * T + 64 <= a.features, RELU, v[T]);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const unsigned m = RELU ? __builtin_bit_cast(unsigned, v[T][i]) : magnitude(v[T][i]);
+                        top = top > m ? top : m;
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-            }
-        } else {
-            // the whole row is here (16 features per group in each of 4 lanes): its scale, then its integers
-            float v[NT][16];
-            unsigned top = 0u;
 #pragma unroll
-            for (int T = 0; T < NT; ++T) {
-                finish_linear<ADD>(a, acc[T], ws + 64 * T + 16 * g, bs + 64 * T + 16 * g, now.xs, 64 * T + 16 * g, p,
-                                   64 * T + 64 <= a.features, v[T]);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const unsigned m = magnitude(v[T][i]);
-                    top = top > m ? top : m;
+                for (int off = 16; off < 64; off *= 2) {
+                    const unsigned o = (unsigned)__shfl_xor((int)top, off);
+                    top = top > o ? top : o;
                 }
-                __builtin_amdgcn_sched_barrier(0);  // in turn: 16 sums become 16 values in the same registers
-            }
-#pragma unroll
-            for (int off = 16; off < 64; off *= 2) {
-                const unsigned o = (unsigned)__shfl_xor((int)top, off);
-                top = top > o ? top : o;
-            }
-            const Scale sc = scale_of(top, a.pow2 != 0);
-            const int fp = a.groups * 64;  // width of a row of the output
-            if (live) {
-                if (g == 0) a.out_scale[p] = sc.scale;
+                const Scale sc = scale_of(top, POW2);
+                const bool has_nan = __any(top > 0x7f800000u);
+                const int fp = a.groups * 64;  // width of a row of the output
+                if (live && g == 0) a.out_scale[p] = sc.scale;
 #pragma unroll
                 for (int T = 0; T < NT; ++T) {
                     if (T < a.groups) {
-                        unsigned o[4], bits = 0u;
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            float t[4];
-#pragma unroll
-                            for (int b = 0; b < 4; ++b) {
-                                t[b] = v[T][4 * w + b] * sc.inv;
-                                bits |= v[T][4 * w + b] > 0.f ? 1u << (4 * w + b) : 0u;
-                            }
-                            o[w] = round4(t);
+                        const uint4 o = round16<POW2>(v[T], sc.inv);
+                        if (live) *(uint4*)((signed char*)a.out + p * fp + 64 * T + 16 * g) = o;
+                        if (a.out_mask) {
+                            const unsigned bits = positive_bits<RELU>(v[T], has_nan);
+                            if (live) *(unsigned short*)(a.out_mask + p * (fp / 8) + 8 * T + 2 * g) = (unsigned short)bits;
                         }
-                        if (sc.inv == 0.f) o[0] = o[1] = o[2] = o[3] = 0u;
-                        *(uint4*)((signed char*)a.out + p * fp + 64 * T + 16 * g) = make_uint4(o[0], o[1], o[2], o[3]);
-                        if (a.out_mask) *(unsigned short*)(a.out_mask + p * (fp / 8) + 8 * T + 2 * g) = (unsigned short)bits;
                     }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
         }
@@ -379,11 +424,14 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
             const int64_t tile1 = last ? tile + stride : tile;
             const int s1 = last ? 0 : s0 + CH;
             if (s0 == 0) {
-                side[0] = side[1];
 #pragma unroll
-                for (int T = 0; T < NT; ++T)
+                for (int j = 0; j < P; ++j) {
+                    side[0][j] = side[1][j];
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) acc[T][u] = typename Op::Acc{};
+                    for (int T = 0; T < NT; ++T)
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) acc[j][T][u] = typename Op::Acc{};
+                }
             }
             fetch(tile1 < tiles ? tile1 : tile, s1, raw[h ^ 1]);
             multiply(s0, raw[h]);
@@ -395,16 +443,16 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
 
 constexpr int kLdsBytes = 160 * 1024;
 
-template <class Op, int OUT, int NT, int CH, bool ADD>
+template <class Op, int OUT, int NT, int CH, int P, bool ADD>
 int launch_resident(const LinearArgs& a, const char* what, hipStream_t st) {
     const size_t lds = channel_bytes<NT>() + (size_t)NT * a.steps * 4096;
-    auto kernel = linear_resident_kernel<Op, OUT, NT, CH, ADD>;
+    auto kernel = linear_resident_kernel<Op, OUT, NT, CH, P, ADD>;
     // (the limit is an attribute of the function on every device; asking again costs nothing)
     const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes);
     if (e != hipSuccess) return NERF_FAIL((int)e, "%s: %s", what, hipGetErrorString(e));
     int cus = device_cu_count();
     if (cus <= 0) cus = 256;
-    const int64_t tiles = (a.n + kTile - 1) / kTile;
+    const int64_t tiles = (a.n + 16 * P - 1) / (16 * P);
     const int fblocks = (a.groups + NT - 1) / NT;
     int64_t blocks = (tiles + kResidentThreads / 64 - 1) / (kResidentThreads / 64);
     const int64_t most = cus / fblocks > 0 ? cus / fblocks : 1;

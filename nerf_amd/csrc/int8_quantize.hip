@@ -47,10 +47,10 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const void* __restri
             float lo[4], hi[4];
             unsigned bits = 0u;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) lo[i] = w[i] * sc.inv, hi[i] = w[i + 4] * sc.inv;
+            for (int i = 0; i < 4; ++i) lo[i] = w[i] * sc.inv + kRoundAt, hi[i] = w[i + 4] * sc.inv + kRoundAt;
 #pragma unroll
             for (int i = 0; i < 8; ++i) bits |= w[i] > 0.f ? 1u << i : 0u;
-            *(uint2*)(qr + 8 * c) = sc.inv == 0.f ? make_uint2(0u, 0u) : make_uint2(round4(lo), round4(hi));
+            *(uint2*)(qr + 8 * c) = sc.inv == 0.f ? make_uint2(0u, 0u) : make_uint2(low_bytes(lo), low_bytes(hi));
             if (mr) mr[c] = (unsigned char)bits;
         };
         if constexpr (NV > 0) {

@@ -235,9 +235,14 @@ def test_linear_int8(gpu, n, k, m, dtype, pow2):
         assert got.dtype == t
         # sum, two scales, bias and addend: five roundings of 2^-24, each of at most `mag` (1 + 2^-22); then the type's
         close(got, want, mag * 5.001 * 2.0 ** -24 + half * (want.abs() + mag * 2.0 ** -20) + TINY[t], (n, k, m, dtype))
-    # by the formula in fp32, bit for bit
-    y = (sums.float() * ws.float()) * rows.scale[:, None] + b
-    assert torch.equal(ops.linear_int8(rows, packed, b), y)
+    # by the formula in fp32: the sum and its product with the channel scale are rounded, then the product with
+    # the row scale plus the bias once (exact in 64 bits but for a last rounding there, which can move the
+    # one to fp32 by a step when it falls on a tie: never for power-of-two scales here)
+    y64 = (sums.float() * ws.float()).double() * rows.scale.double()[:, None] + b.double()
+    y = ops.linear_int8(rows, packed, b)
+    assert float((y.double() - y64).abs().sub(2.0 ** -24 * (1 + 2.0 ** -20) * y64.abs()).max()) <= 1e-40
+    if pow2:
+        assert torch.equal(y, (sums.float() * ws.float()) * rows.scale[:, None] + b)
     # and in 8 bits again: as if y had been stored in fp32 and quantised
     y = torch.relu(y)
     for p2 in (False, True):
