@@ -41,8 +41,10 @@ DEV bf16x8 tr_operand(const char* img, int half, int lane) {
     return __builtin_bit_cast(bf16x8, v);
 }
 
-template <int DT, int MT>
-__global__ __launch_bounds__(256) void grad_weight_kernel(GradWeightArgs a) {
+// EVEN: rows of dz are a whole number of 8-feature pieces, so that every piece is inside its row or wholly
+// behind it (and then any piece of the row will do: its columns are not stored).
+template <int DT, int MT, bool EVEN>
+__global__ __launch_bounds__(256, 2) void grad_weight_kernel(GradWeightArgs a) {
     typedef typename Elem<DT>::T T;
     constexpr int N = Terms<DT>::N, YT = MT / 32, XT = kTileK / 32;
     constexpr int kChunks = MT >= 64 ? MT / 64 : 1;   // pieces of 8 features of dz per thread and stage
@@ -60,7 +62,8 @@ __global__ __launch_bounds__(256) void grad_weight_kernel(GradWeightArgs a) {
     const int kb = blk % a.kblocks, mb = blk / a.kblocks;
     const int64_t lo = slice * a.rows_per;
     const int64_t hi = lo + a.rows_per < a.n ? lo + a.rows_per : a.n;
-    const int64_t stages = hi > lo ? (hi - lo + kStageRows - 1) / kStageRows : 0;
+    const int64_t stages = hi > lo ? (hi - lo) / kStageRows : 0;  // whole ones; what is left is done last
+    const int left = hi > lo ? (int)((hi - lo) % kStageRows) : 0;
 
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     // this thread's piece of the rows: 16 integers
@@ -86,19 +89,23 @@ __global__ __launch_bounds__(256) void grad_weight_kernel(GradWeightArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum[i][j] = 0.f;
 
-    auto fetch = [&](int64_t st, Held& h) {
-        const int64_t row0 = lo + st * kStageRows;
-        const int64_t rx = row0 + xp < hi ? row0 + xp : hi - 1;   // a row behind the last: its dz is taken as zero
+    // rows row0 + 0 .. 31; those behind `most` repeat it
+    auto fetch = [&](int64_t row0, int64_t most, Held& h) {
+        const int64_t rx = row0 + xp < most ? row0 + xp : most;
         h.x = *(const i32x4*)(a.q + rx * a.kp + xc);
         if (has_y) {
-            const int64_t ry = row0 + yp < hi ? row0 + yp : hi - 1;
+            const int64_t ry = row0 + yp < most ? row0 + yp : most;
             h.s = a.scale[ry];
             const T* src = (const T*)a.dz + ry * a.lddz;
 #pragma unroll
-            for (int i = 0; i < kChunks; ++i) h.y[i] = load8<T>(src, mb * MT + (yt0 + 2 * i) * 32 + yq * 8, a.m, y_whole);
+            for (int i = 0; i < kChunks; ++i) {
+                const int col = mb * MT + (yt0 + 2 * i) * 32 + yq * 8;
+                if constexpr (EVEN) h.y[i] = load8<T>(src, col < a.m ? col : 0, a.m, true);
+                else h.y[i] = load8<T>(src, col, a.m, y_whole);
+            }
         }
     };
-    auto stage = [&](int64_t st, const Held& h, char* buf) {
+    auto stage = [&](const Held& h, char* buf, bool on) {
         {
             bf16x8 o[2];
 #pragma unroll
@@ -110,7 +117,7 @@ __global__ __launch_bounds__(256) void grad_weight_kernel(GradWeightArgs a) {
             *(bf16x8*)(dst + 16) = o[1];
         }
         if (has_y) {
-            const bool on = lo + st * kStageRows + yp < hi;
+            const float xs = on ? h.s : 0.f;
 #pragma unroll
             for (int i = 0; i < kChunks; ++i) {
                 float v[8];
@@ -119,7 +126,7 @@ __global__ __launch_bounds__(256) void grad_weight_kernel(GradWeightArgs a) {
                 for (int j = 0; j < 8; ++j) {
                     v[j] = on ? v[j] : 0.f;
                     sum[i][j] += v[j];
-                    v[j] *= on ? h.s : 0.f;
+                    v[j] *= xs;
                 }
                 bf16x8 o[N];
                 split_bf16<N>(v, o);
@@ -139,34 +146,46 @@ __global__ __launch_bounds__(256) void grad_weight_kernel(GradWeightArgs a) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
 
+    auto multiply = [&](const char* buf) {
 #pragma unroll
-    for (int d = 0; d < D; ++d)
-        if (d < stages) fetch(d, held[d]);
-    if (stages > 0) stage(0, held[0], lds);
-    __syncthreads();
-    for (int64_t st0 = 0; st0 < stages; st0 += D) {
+        for (int half = 0; half < 2; ++half) {
+            bf16x8 xo[AX];
 #pragma unroll
-        for (int d = 0; d < D; ++d) {
-            const int64_t st = st0 + d;
-            if (st >= stages) break;
-            const char* buf = lds + (d & 1) * kStage;
-            if (st + D < stages) fetch(st + D, held[d]);
+            for (int x = 0; x < AX; ++x) xo[x] = tr_operand(buf + (wx + x) * kImg, half, lane);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                bf16x8 xo[AX];
+            for (int s = 0; s < N; ++s)
 #pragma unroll
-                for (int x = 0; x < AX; ++x) xo[x] = tr_operand(buf + (wx + x) * kImg, half, lane);
+                for (int y = 0; y < AY; ++y) {
+                    const bf16x8 yo = tr_operand(buf + (XT + s * YT + wy + y) * kImg, half, lane);
 #pragma unroll
-                for (int s = 0; s < N; ++s)
+                    for (int x = 0; x < AX; ++x) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xo[x], yo, acc[x][y], 0, 0, 0);
+                }
+        }
+    };
+    // every fetch is made, also of stages that do not exist (they repeat the last row): a wait for older
+    // loads counts the younger ones
+    if (hi > lo) {
 #pragma unroll
-                    for (int y = 0; y < AY; ++y) {
-                        const bf16x8 yo = tr_operand(buf + (XT + s * YT + wy + y) * kImg, half, lane);
+        for (int d = 0; d < D; ++d) fetch(lo + d * kStageRows, hi - 1, held[d]);
+        if (stages > 0) stage(held[0], lds, true);
+        __syncthreads();
+        for (int64_t st0 = 0; st0 < stages; st0 += D) {
 #pragma unroll
-                        for (int x = 0; x < AX; ++x) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xo[x], yo, acc[x][y], 0, 0, 0);
-                    }
+            for (int d = 0; d < D; ++d) {
+                const int64_t st = st0 + d;
+                if (st >= stages) break;
+                fetch(lo + (st + D) * kStageRows, hi - 1, held[d]);
+                multiply(lds + (d & 1) * kStage);
+                // into the buffer that was read in the turn before this one
+                if (st + 1 < stages) stage(held[(d + 1) % D], lds + ((d + 1) & 1) * kStage, true);
+                __syncthreads();
             }
-            // into the buffer that was read in the turn before this one
-            if (st + 1 < stages) stage(st + 1, held[(d + 1) % D], lds + ((d + 1) & 1) * kStage);
+        }
+        if (left > 0) {
+            fetch(lo + stages * kStageRows, hi - 1, held[0]);
+            stage(held[0], lds, yp < left);
+            __syncthreads();
+            multiply(lds);
             __syncthreads();
         }
     }
@@ -281,8 +300,9 @@ NERF_API int nerf_linear_int8_grad_weight(const signed char* q, const float* sca
     hipStream_t st = as_stream(stream);
 #define NERF_W(DT)                                                                     \
     do {                                                                               \
-        if (c.tile_m == 32) grad_weight_kernel<DT, 32><<<grid, 256, 0, st>>>(a);       \
-        else grad_weight_kernel<DT, 128><<<grid, 256, 0, st>>>(a);                     \
+        if (c.tile_m == 32) grad_weight_kernel<DT, 32, false><<<grid, 256, 0, st>>>(a);     \
+        else if (m % 8 == 0) grad_weight_kernel<DT, 128, true><<<grid, 256, 0, st>>>(a);    \
+        else grad_weight_kernel<DT, 128, false><<<grid, 256, 0, st>>>(a);                   \
     } while (0)
     if (dtype == NERF_F32) NERF_W(NERF_F32);
     else if (dtype == NERF_F16) NERF_W(NERF_F16);
