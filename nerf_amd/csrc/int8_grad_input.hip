@@ -19,6 +19,10 @@ static int resident(const LinearArgs& a, const char* what, hipStream_t st) {
 template <int DT>
 static int launch(const LinearArgs& a, const char* what, hipStream_t st) {
     const int nt = resident_groups(a);
+    if constexpr (DT == NERF_BF16) {
+        if (a.n >= kResidentRows && (nt == 0 || a.groups > nt) && a.width % 32 == 0 && a.lddz % 8 == 0 && ((uintptr_t)a.dz & 15) == 0)
+            return launch_streamed<Bf16Op<DT, true>, DT, false>(a, what, st);
+    }
     if (a.n < kResidentRows || nt == 0) return launch_direct<Bf16Op<DT, false>, DT, false>(a, what, st);
     if (nt == 4) return resident<DT, 4>(a, what, st);
     if (nt == 2) return resident<DT, 2>(a, what, st);
@@ -44,7 +48,7 @@ NERF_API int nerf_linear_int8_grad_input(const void* dz, int dtype, int64_t n, i
                  "%s: misaligned pointer", what);
     const PackedLayout lay(k, m, true);
     LinearArgs a{};
-    a.frags = (const char*)packed + lay.frags_t, a.groups = lay.kp / 64, a.steps = lay.mp / 32, a.n = n;
+    a.frags = (const char*)packed + lay.frags_t, a.groups = lay.kp / 64, a.steps = (m + 31) / 32, a.frag_steps = lay.mp / 32, a.n = n;
     a.dz = dz, a.lddz = lddz, a.width = m, a.features = k, a.mask = mask, a.out = dx, a.ldout = lddx;
     hipStream_t st = as_stream(stream);
     if (dtype == NERF_F32) return launch<NERF_F32>(a, what, st);

@@ -26,7 +26,8 @@ template <int OUT, bool ADD>
 static int launch(const LinearArgs& a, const char* what, hipStream_t st) {
     const int nt = resident_groups(a);
     if constexpr (OUT < TO_INT8) {
-        if (a.n < kResidentRows || nt == 0) return launch_direct<Int8Op, OUT, ADD>(a, what, st);
+        if (a.n < kResidentRows) return launch_direct<Int8Op, OUT, ADD>(a, what, st);
+        if (nt == 0 || a.groups > nt) return launch_streamed<Int8Op, OUT, ADD>(a, what, st);
     }
     if (nt == 4) return resident<OUT, 4, ADD>(a, what, st);
     if (nt == 2) return resident<OUT, 2, ADD>(a, what, st);
@@ -50,7 +51,7 @@ static int linear_args(LinearArgs& a, const char* what, const signed char* q, co
                      (!addend || ((uintptr_t)addend & (dtype_size(addend_dtype) - 1)) == 0),
                  "%s: misaligned pointer", what);
     const PackedLayout lay(k, m, false);
-    a.frags = (const char*)packed + lay.frags, a.groups = lay.mp / 64, a.steps = lay.kp / 64, a.n = n;
+    a.frags = (const char*)packed + lay.frags, a.groups = lay.mp / 64, a.steps = a.frag_steps = lay.kp / 64, a.n = n;
     a.q = q, a.scale = scale, a.features = m, a.wscale = (const float*)packed, a.bias = bias;
     a.addend = addend, a.add_dtype = addend_dtype, a.ldadd = ldadd, a.relu = relu;
     return 0;

@@ -7,13 +7,15 @@
 // 16 neighbouring features of one point in a lane.
 #pragma once
 #include "int8_common.h"
+#include "mlp_common.h"
 
 namespace nerf {
 namespace i8 {
 
 struct LinearArgs {
     const char* frags;     // this product's fragments
-    int groups, steps;     // groups of 64 features, steps of 64 integers (32 bf16)
+    int groups, steps;     // groups of 64 features, steps of 64 integers (32 bf16) of the rows
+    int frag_steps;        // ... of the fragments (bf16: one more where the rows end in the first half of 64)
     int64_t n;
     // the rows: q and scale, or dz
     const signed char* q;
@@ -54,6 +56,7 @@ struct Int8Op {
         i32x4 v;
         DEV B(const Raw& r) : v(r) {}
     };
+    static DEV Raw raw_of(i32x4 w) { return w; }
     static DEV Acc mma(i32x4 w, const B& b, Acc c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(w, b.v, c, 0, 0, 0); }
 };
 
@@ -67,6 +70,11 @@ struct Bf16Op {
     static constexpr int N = Terms<DT>::N;
     static DEV Raw fetch(const LinearArgs& a, int64_t p, int s, int g) {
         return load8<T>((const T*)a.dz + p * a.lddz, 32 * s + 8 * g, a.width, EVEN || 32 * s + 32 <= a.width);
+    }
+    static DEV Raw raw_of(i32x4 w) {  // 16-bit types
+        Raw r;
+        r.w[0] = w;
+        return r;
     }
     struct B {
         bf16x8 v[N];
@@ -216,7 +224,7 @@ __global__ __launch_bounds__(256) void linear_direct_kernel(LinearArgs a) {
         const int64_t p = p0 + 16 * j + r;
         row[j] = p < a.n ? p : a.n - 1;  // a lane behind the last row repeats it and stores nothing
     }
-    const char* w = a.frags + (size_t)T * a.steps * 4096 + lane * 16;
+    const char* w = a.frags + (size_t)T * a.frag_steps * 4096 + lane * 16;
     for (int s = 0; s < a.steps; ++s, w += 4096) {
         typename Op::Raw raw[P];
 #pragma unroll
@@ -276,11 +284,11 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
 
     // fragments [group][step] -> LDS [step][group]; groups behind the last are zeros
     {
-        const int have = (a.groups - T0 < NT ? a.groups - T0 : NT) * a.steps * 256, all = NT * a.steps * 256;
-        const i32x4* src = (const i32x4*)(a.frags + (size_t)T0 * a.steps * 4096);
-        for (int i = threadIdx.x; i < all; i += kResidentThreads) {
+        const i32x4* src = (const i32x4*)(a.frags + (size_t)T0 * a.frag_steps * 4096);
+        for (int i = threadIdx.x; i < NT * a.steps * 256; i += kResidentThreads) {
             const int T = i / (a.steps * 256), s = (i >> 8) - T * a.steps;
-            *(i32x4*)(wl + ((s * NT + T) * 256 + (i & 255)) * 16) = i < have ? src[i] : i32x4{0, 0, 0, 0};
+            *(i32x4*)(wl + ((s * NT + T) * 256 + (i & 255)) * 16) =
+                T0 + T < a.groups ? src[(T * a.frag_steps + s) * 256 + (i & 255)] : i32x4{0, 0, 0, 0};
         }
         if constexpr (Op::kInt8) stage_channels(a, ws, bs, 64 * T0, NT * 64);
     }
@@ -441,6 +449,112 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
     }
 }
 
+// Weights that do not fit LDS: a workgroup forms a tile of 256 features x 256 points, a wave 128 x 64 of
+// it (128 registers of sums).  The contraction goes through a ring of four stages of one step (16
+// fragments of weights, 16 of rows: 32 KiB), copied from global memory to LDS without passing
+// registers, three stages ahead; per stage a wave reads 12 fragments for 32 products, so the matrix
+// unit and not LDS sets the pace.  Rows must be 16-byte aligned and end with a step.  Workgroups 8 apart
+// run on the same die: they take the feature blocks of one block of rows in turn, which the die's L2
+// then holds.
+constexpr int kStreamThreads = 512, kStreamStages = 4, kStreamStage = 32 * 1024;
+
+template <class Op, int OUT, bool ADD>
+__global__ __launch_bounds__(kStreamThreads) void linear_streamed_kernel(LinearArgs a, int fblocks, int64_t pblocks) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    float* const ws = (float*)lds;
+    float* const bs = ws + 256;
+    char* const ring = lds + 2 * 256 * 4;
+    const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int fb = (int)(blockIdx.x / 8 % fblocks);
+    const int64_t pb = (int64_t)(blockIdx.x / 8 / fblocks) * 8 + (blockIdx.x & 7);
+    if (pb >= pblocks) return;  // the whole workgroup
+    const int T0 = 4 * fb;
+
+    // this wave's four copies of a stage: fragments of weights (waves 0-3), of rows (waves 4-7)
+    const char* src[4];
+    const int step = wave < 4 ? 4096 : 64;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (wave < 4) {
+            const int T = T0 + wave < a.groups ? T0 + wave : a.groups - 1;  // a group behind the last is not stored
+            src[i] = a.frags + (size_t)T * a.frag_steps * 4096 + i * 1024 + lane * 16;
+        } else {
+            int64_t p = pb * 256 + ((wave - 4) * 4 + i) * 16 + r;
+            if (p >= a.n) p = a.n - 1;
+            if constexpr (Op::kInt8) src[i] = (const char*)a.q + p * a.steps * 64 + 16 * g;
+            else src[i] = (const char*)a.dz + p * a.lddz * 2 + 16 * g;
+        }
+    }
+    auto issue = [&](int s) {
+        char* dst = ring + (s % kStreamStages) * kStreamStage + wave * 4096;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) glds16_untracked(src[i] + (int64_t)s * step, dst + i * 1024);
+    };
+
+    if constexpr (Op::kInt8) {
+        stage_channels(a, ws, bs, 64 * T0, 256);  // read behind the barriers of the loop
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing but the copies is counted from here on
+    }
+    const int wf = wave & 1, wp = wave >> 1;
+    typename Op::Acc acc[4][2][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) acc[j][t][u] = typename Op::Acc{};
+#pragma unroll
+    for (int s = 0; s < kStreamStages - 1; ++s)
+        if (s < a.steps) issue(s);
+    for (int s = 0; s < a.steps; ++s) {
+        // this wave's copies of stage s have arrived (two younger stages of four may be on their way), then everyone's
+        const int younger = a.steps - 1 - s;
+        if (younger >= 2) wait_vmcnt_n(8);
+        else if (younger == 1) wait_vmcnt_n(4);
+        else wait_vmcnt_n(0);
+        // (lgkmcnt: this wave's reads of the stage that is overwritten next have arrived)
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (s + kStreamStages - 1 < a.steps) issue(s + kStreamStages - 1);
+        const char* st = ring + (s % kStreamStages) * kStreamStage + lane * 16;
+        const char* wl = st + wf * 8 * 1024;
+        const char* xl = st + 16 * 1024 + wp * 4 * 1024;
+        const auto rows = [&](int j) { return typename Op::B(Op::raw_of(*(const i32x4*)(xl + j * 1024))); };
+        const typename Op::B b[4] = {rows(0), rows(1), rows(2), rows(3)};
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const i32x4 wfr = *(const i32x4*)(wl + (4 * t + u) * 1024);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j][t][u] = Op::mma(wfr, b[j], acc[j][t][u]);
+            }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int64_t p = pb * 256 + (wp * 4 + j) * 16 + r;
+        const bool live = p < a.n;
+        const int64_t pc = live ? p : a.n - 1;
+        float xs = 0.f;
+        if constexpr (Op::kInt8) xs = a.scale[pc];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int T = 2 * wf + t, f = 64 * (T0 + T) + 16 * g;
+            const bool whole = 64 * (T0 + T) + 64 <= a.features;
+            if (T0 + T < a.groups) {
+                if constexpr (Op::kInt8) {
+                    float v[16];
+                    finish_linear<ADD>(a, acc[j][t], ws + 64 * T + 16 * g, bs + 64 * T + 16 * g, xs, f, pc, whole, a.relu != 0, v);
+                    if (live) put<OUT>(a, pc, f, whole, v);
+                } else if (live) {
+                    put_grad<OUT>(a, acc[j][t], f, pc, whole, mask_bits(a, pc, f));
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+}
+
 constexpr int kLdsBytes = 160 * 1024;
 
 template <class Op, int OUT, int NT, int CH, int P, bool ADD>
@@ -458,6 +572,19 @@ int launch_resident(const LinearArgs& a, const char* what, hipStream_t st) {
     const int64_t most = cus / fblocks > 0 ? cus / fblocks : 1;
     if (blocks > most) blocks = most;
     kernel<<<dim3((unsigned)blocks, (unsigned)fblocks), kResidentThreads, lds, st>>>(a, tiles);
+    return check_launch(what);
+}
+
+template <class Op, int OUT, bool ADD>
+int launch_streamed(const LinearArgs& a, const char* what, hipStream_t st) {
+    constexpr size_t lds = 2 * 256 * 4 + kStreamStages * kStreamStage;
+    auto kernel = linear_streamed_kernel<Op, OUT, ADD>;
+    const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes);
+    if (e != hipSuccess) return NERF_FAIL((int)e, "%s: %s", what, hipGetErrorString(e));
+    const int fblocks = (a.groups + 3) / 4;
+    const int64_t pblocks = (a.n + 255) / 256, grid = (pblocks + 7) / 8 * 8 * fblocks;
+    if (grid >= (1LL << 23)) return NERF_FAIL(NERF_E_UNSUPPORTED, "%s: too many rows", what);  // fewer than 2^32 work items
+    kernel<<<(unsigned)grid, kStreamThreads, lds, st>>>(a, fblocks, pblocks);
     return check_launch(what);
 }
 
