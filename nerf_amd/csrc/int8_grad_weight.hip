@@ -1,11 +1,11 @@
 // nerf_linear_int8_grad_weight: dW[f][j] = sum over rows i of q[i][f] (s_i dz[i][j]) and db[j] = sum of
 // dz[i][j], from the 8-bit rows a forward pass kept.  Formats: int8_common.h.
 //
-// The contraction runs over the rows, which lie far apart in memory for both operands: a stage of 32
+// The contraction runs over the rows, which lie far apart in memory for both operands: a stage of 32 or 64
 // rows goes through registers into LDS as bf16 images [row][32 features] and is read back transposed
-// (ds_read_b64_tr_b16) as the operands of v_mfma_f32_32x32x16_bf16.  An integer is exact in bf16; s_i, a
-// power of two, moves only the exponent of dz, so dz times it is the exact sum of 1, 2 or 3 bf16 terms
-// (bf16, fp16, fp32) and every product is exact; sums are fp32.
+// (ds_read_b64_tr_b16) as the operands of v_mfma_f32_32x32x16_bf16.  An integer times s_i, a power of two, is
+// exact in bf16 (the scale goes with the integers: bf16 dz then passes untouched), dz is the exact sum
+// of 1, 2 or 3 bf16 terms (bf16, fp16, fp32), so every product is exact; sums are fp32.
 // A workgroup owns a tile of dW and a slice of the rows.  Slices are joined by a second kernel in slice
 // order (no atomics: the same inputs give the same bits).
 #include "int8_common.h"
@@ -16,16 +16,12 @@ namespace i8 {
 typedef short short4v __attribute__((__vector_size__(4 * sizeof(short))));
 typedef short short8 __attribute__((ext_vector_type(8)));
 
-constexpr int kTileK = 128;       // input features of a workgroup's tile
-constexpr int kStageRows = 32;
-constexpr int kImg = kStageRows * 64;  // bytes of the image of 32 features: [32 rows][32 bf16]
-
 struct GradWeightArgs {
     const signed char* q;
     const float* scale;
     const void* dz;
     int64_t n, lddz, rows_per;  // rows of a slice
-    int k, kp, m, kblocks, mblocks, slices;
+    int k, kp, m, kblocks, mblocks, slices;  // blocks: of the tile's features
     float* out;                 // slice s: dW at out + s * stride
     float* out_db;              //          db at out_db + s * stride
     size_t stride;
@@ -41,18 +37,24 @@ DEV bf16x8 tr_operand(const char* img, int half, int lane) {
     return __builtin_bit_cast(bf16x8, v);
 }
 
+// KT x MT features of dW by four waves, stages of R rows, D of them held ahead in registers (even: the LDS
+// buffer of a turn is then known when compiling).
 // EVEN: rows of dz are a whole number of 8-feature pieces, so that every piece is inside its row or wholly
 // behind it (and then any piece of the row will do: its columns are not stored).
-template <int DT, int MT, bool EVEN>
+template <int DT, int KT, int MT, int R, int D, bool EVEN>
 __global__ __launch_bounds__(256, 2) void grad_weight_kernel(GradWeightArgs a) {
     typedef typename Elem<DT>::T T;
-    constexpr int N = Terms<DT>::N, YT = MT / 32, XT = kTileK / 32;
-    constexpr int kChunks = MT >= 64 ? MT / 64 : 1;   // pieces of 8 features of dz per thread and stage
+    constexpr int N = Terms<DT>::N, YT = MT / 32, XT = KT / 32;
+    constexpr int kImg = R * 64;  // bytes of the image of 32 features: [R rows][32 bf16]
     constexpr int kStage = (XT + N * YT) * kImg;
-    constexpr int AX = MT == 32 ? 1 : 2, AY = MT == 32 ? 1 : 2;  // 32 x 32 tiles of a wave
-    constexpr int D = DT == NERF_F32 ? 2 : 4;  // even: the LDS buffer of a turn is then known when compiling
-    static_assert(MT == 32 || MT == 128, "tile");
+    constexpr int kXPieces = R * KT / 16, kYPieces = R * MT / 8;   // 16 integers, 8 elements of dz
+    constexpr int CX = (kXPieces + 255) / 256, CY = (kYPieces + 255) / 256;  // of a thread
+    // waves along k and m, and 32 x 32 tiles of a wave
+    constexpr int WX = MT == 32 ? 4 : KT == 128 ? 2 : 1, WY = 4 / WX, AX = XT / WX, AY = YT / WY;
+    constexpr int kRowBits = R == 64 ? 6 : 5, kTileBits = KT == 128 ? 2 : 1;
+    static_assert((R == 32 || R == 64) && (KT == 64 || KT == 128) && AX >= 1 && AY >= 1 && D % 2 == 0, "shapes");
     __shared__ __attribute__((aligned(16))) char lds[2 * kStage];
+    static_assert(2 * kStage >= R * MT * 4, "the sums of dz meet in LDS");
 
     // workgroups 8 apart run on the same die and share its L2: the tiles of one slice read the same rows
     const int nb = a.kblocks * a.mblocks;
@@ -62,82 +64,97 @@ __global__ __launch_bounds__(256, 2) void grad_weight_kernel(GradWeightArgs a) {
     const int kb = blk % a.kblocks, mb = blk / a.kblocks;
     const int64_t lo = slice * a.rows_per;
     const int64_t hi = lo + a.rows_per < a.n ? lo + a.rows_per : a.n;
-    const int64_t stages = hi > lo ? (hi - lo) / kStageRows : 0;  // whole ones; what is left is done last
-    const int left = hi > lo ? (int)((hi - lo) % kStageRows) : 0;
+    const int64_t stages = hi > lo ? (hi - lo) / R : 0;  // whole ones; what is left is done last
+    const int left = hi > lo ? (int)((hi - lo) % R) : 0;
 
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    // this thread's piece of the rows: 16 integers
-    const int xh = t & 1, xt = (lane >> 4) & 3, xp = wave * 8 + ((lane >> 1) & 7);
-    const int xcol = kb * kTileK + xt * 32 + xh * 16;
-    // ... and of dz: 8 features of row yp, in the images yt0 + 2 i
-    const int yq = t & 3, yp = (t >> 2) & 31, yt0 = t >> 7;
-    const bool has_y = MT >= 64 || t < 128;
-
-    const int xc = xcol < a.kp ? xcol : 0;   // columns behind the last are computed and not stored
+    // Piece e of the rows: half of an image's 32 features (bit 0), 3 bits of the row, the image, the other bits of
+    // the row: a wave reads runs of a row and writes LDS without conflicts.  Piece e of dz: a quarter of an
+    // image (2 bits), the row, the image.
+    auto x_half = [&](int e) { return e & 1; };
+    auto x_img = [&](int e) { return (e >> 4) & (XT - 1); };
+    auto x_row = [&](int e) { return ((e >> 1) & 7) | (e >> (4 + kTileBits)) << 3; };
+    auto y_row = [&](int e) { return (e >> 2) & (R - 1); };
+    auto y_img = [&](int e) { return e >> (2 + kRowBits); };
+    const int yq = t & 3;
+    const bool has_x = kXPieces >= 256 || t < kXPieces, has_y = kYPieces >= 256 || t < kYPieces;
     const bool y_whole = mb * MT + MT <= a.m;
 
-    // Stages D - 1 turns ahead are on their way in registers: one stage of a workgroup is only some 12 KiB.
     struct Held {
-        i32x4 x;
-        Raw8<T> y[kChunks];
-        float s;
+        i32x4 x[CX];
+        float s[CX];
+        Raw8<T> y[CY];
     };
     Held held[D];
-    float sum[kChunks][8];
+    float sum[CY][8];
 #pragma unroll
-    for (int i = 0; i < kChunks; ++i)
+    for (int i = 0; i < CY; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum[i][j] = 0.f;
 
-    // rows row0 + 0 .. 31; those behind `most` repeat it
+    // rows from row0; those behind `most` repeat it
     auto fetch = [&](int64_t row0, int64_t most, Held& h) {
-        const int64_t rx = row0 + xp < most ? row0 + xp : most;
-        h.x = *(const i32x4*)(a.q + rx * a.kp + xc);
-        if (has_y) {
-            const int64_t ry = row0 + yp < most ? row0 + yp : most;
-            h.s = a.scale[ry];
-            const T* src = (const T*)a.dz + ry * a.lddz;
+        if (has_x) {
 #pragma unroll
-            for (int i = 0; i < kChunks; ++i) {
-                const int col = mb * MT + (yt0 + 2 * i) * 32 + yq * 8;
+            for (int i = 0; i < CX; ++i) {
+                const int e = t + 256 * i, col = kb * KT + x_img(e) * 32 + x_half(e) * 16;
+                const int64_t row = row0 + x_row(e) < most ? row0 + x_row(e) : most;
+                h.x[i] = *(const i32x4*)(a.q + row * a.kp + (col < a.kp ? col : 0));  // (behind the last: not stored)
+                h.s[i] = a.scale[row];
+            }
+        }
+        if (has_y) {
+#pragma unroll
+            for (int i = 0; i < CY; ++i) {
+                const int e = t + 256 * i, col = mb * MT + y_img(e) * 32 + yq * 8;
+                const int64_t row = row0 + y_row(e) < most ? row0 + y_row(e) : most;
+                const T* src = (const T*)a.dz + row * a.lddz;
                 if constexpr (EVEN) h.y[i] = load8<T>(src, col < a.m ? col : 0, a.m, true);
                 else h.y[i] = load8<T>(src, col, a.m, y_whole);
             }
         }
     };
-    auto stage = [&](const Held& h, char* buf, bool on) {
-        {
-            bf16x8 o[2];
+    // ... into LDS as bf16; of a last stage only the first `rows`
+    auto stage = [&](const Held& h, char* buf, int rows) {
+        if (has_x) {
 #pragma unroll
-            for (int w = 0; w < 4; ++w)
+            for (int i = 0; i < CX; ++i) {
+                const int e = t + 256 * i;
+                const float xs = x_row(e) < rows ? h.s[i] : 0.f;
+                bf16x8 o[2];
 #pragma unroll
-                for (int b = 0; b < 4; ++b) o[w >> 1][(w & 1) * 4 + b] = (__bf16)(float)((h.x[w] << (24 - 8 * b)) >> 24);
-            char* dst = buf + xt * kImg + xp * 64 + xh * 32;
-            *(bf16x8*)dst = o[0];
-            *(bf16x8*)(dst + 16) = o[1];
+                for (int w = 0; w < 4; ++w)
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) o[w >> 1][(w & 1) * 4 + b] = (__bf16)((float)((h.x[i][w] << (24 - 8 * b)) >> 24) * xs);
+                char* dst = buf + x_img(e) * kImg + x_row(e) * 64 + x_half(e) * 32;
+                *(bf16x8*)dst = o[0];
+                *(bf16x8*)(dst + 16) = o[1];
+            }
         }
         if (has_y) {
-            const float xs = on ? h.s : 0.f;
 #pragma unroll
-            for (int i = 0; i < kChunks; ++i) {
-                float v[8];
-                to_float(h.y[i], v);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    v[j] = on ? v[j] : 0.f;
-                    sum[i][j] += v[j];
-                    v[j] *= xs;
-                }
+            for (int i = 0; i < CY; ++i) {
+                const int e = t + 256 * i;
+                const bool on = y_row(e) < rows;
                 bf16x8 o[N];
-                split_bf16<N>(v, o);
+                if (DT != NERF_BF16 || kb == 0) {
+                    float v[8];
+                    to_float(h.y[i], v);
 #pragma unroll
-                for (int s = 0; s < N; ++s)
-                    *(bf16x8*)(buf + (XT + s * YT + yt0 + 2 * i) * kImg + yp * 64 + yq * 16) = o[s];
+                    for (int j = 0; j < 8; ++j) {
+                        v[j] = on ? v[j] : 0.f;
+                        sum[i][j] += v[j];
+                    }
+                    if constexpr (DT != NERF_BF16) split_bf16<N>(v, o);
+                }
+                if constexpr (DT == NERF_BF16) o[0] = __builtin_bit_cast(bf16x8, on ? h.y[i].w[0] : i32x4{0, 0, 0, 0});
+#pragma unroll
+                for (int s = 0; s < N; ++s) *(bf16x8*)(buf + (XT + s * YT + y_img(e)) * kImg + y_row(e) * 64 + yq * 16) = o[s];
             }
         }
     };
 
-    const int wx = MT == 32 ? wave : 2 * (wave & 1), wy = MT == 32 ? 0 : 2 * (wave >> 1);
+    const int wx = (wave % WX) * AX, wy = (wave / WX) * AY;
     f32x16 acc[AX][AY];
 #pragma unroll
     for (int x = 0; x < AX; ++x)
@@ -145,10 +162,9 @@ __global__ __launch_bounds__(256, 2) void grad_weight_kernel(GradWeightArgs a) {
         for (int y = 0; y < AY; ++y)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
-
     auto multiply = [&](const char* buf) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+        for (int half = 0; half < R / 16; ++half) {
             bf16x8 xo[AX];
 #pragma unroll
             for (int x = 0; x < AX; ++x) xo[x] = tr_operand(buf + (wx + x) * kImg, half, lane);
@@ -166,24 +182,24 @@ __global__ __launch_bounds__(256, 2) void grad_weight_kernel(GradWeightArgs a) {
     // loads counts the younger ones
     if (hi > lo) {
 #pragma unroll
-        for (int d = 0; d < D; ++d) fetch(lo + d * kStageRows, hi - 1, held[d]);
-        if (stages > 0) stage(held[0], lds, true);
+        for (int d = 0; d < D; ++d) fetch(lo + d * R, hi - 1, held[d]);
+        if (stages > 0) stage(held[0], lds, R);
         __syncthreads();
         for (int64_t st0 = 0; st0 < stages; st0 += D) {
 #pragma unroll
             for (int d = 0; d < D; ++d) {
                 const int64_t st = st0 + d;
                 if (st >= stages) break;
-                fetch(lo + (st + D) * kStageRows, hi - 1, held[d]);
+                fetch(lo + (st + D) * R, hi - 1, held[d]);
                 multiply(lds + (d & 1) * kStage);
                 // into the buffer that was read in the turn before this one
-                if (st + 1 < stages) stage(held[(d + 1) % D], lds + ((d + 1) & 1) * kStage, true);
+                if (st + 1 < stages) stage(held[(d + 1) % D], lds + ((d + 1) & 1) * kStage, R);
                 __syncthreads();
             }
         }
         if (left > 0) {
-            fetch(lo + stages * kStageRows, hi - 1, held[0]);
-            stage(held[0], lds, yp < left);
+            fetch(lo + stages * R, hi - 1, held[0]);
+            stage(held[0], lds, left);
             __syncthreads();
             multiply(lds);
             __syncthreads();
@@ -198,24 +214,105 @@ __global__ __launch_bounds__(256, 2) void grad_weight_kernel(GradWeightArgs a) {
             const int col = mb * MT + (wy + y) * 32 + (lane & 31);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int f = kb * kTileK + (wx + x) * 32 + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5);
+                const int f = kb * KT + (wx + x) * 32 + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5);
                 if (f < a.k && col < a.m) out[(size_t)f * a.m + col] = acc[x][y][r];
             }
         }
     if (kb != 0) return;  // the whole workgroup
-    // db: the 32 row lanes of a feature meet in LDS (free: behind the last barrier), added in row order
-    float* red = (float*)lds;  // [32][MT]
+    // db: the row lanes of a feature meet in LDS (free: behind the last barrier), added in row order
+    float* red = (float*)lds;  // [R][MT]
     if (has_y) {
 #pragma unroll
-        for (int i = 0; i < kChunks; ++i)
+        for (int i = 0; i < CY; ++i) {
+            const int e = t + 256 * i;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) red[yp * MT + (yt0 + 2 * i) * 32 + yq * 8 + j] = sum[i][j];
+            for (int j = 0; j < 8; ++j) red[y_row(e) * MT + y_img(e) * 32 + yq * 8 + j] = sum[i][j];
+        }
     }
     __syncthreads();
     if (t < MT && mb * MT + t < a.m) {
         float s = 0.f;
-        for (int p = 0; p < 32; ++p) s += red[p * MT + t];
+        for (int p = 0; p < R; ++p) s += red[p * MT + t];
         a.out_db[slice * a.stride + mb * MT + t] = s;
+    }
+}
+
+// Up to four outputs (the colour and density heads): a matrix tile would be nearly empty, so a thread owns 16
+// input features, streams its share of the rows past 16 M sums in registers (one conversion and M
+// multiply-adds an integer, which the rows' bytes still outlast) and the workgroup's threads meet in LDS
+// at the end.  blockIdx.y: blocks of 64 pieces of 16 features.
+constexpr int kThinPieces = 64;
+template <int DT, int M>
+__global__ __launch_bounds__(256) void grad_weight_thin_kernel(GradWeightArgs a) {
+    typedef typename Elem<DT>::T T;
+    __shared__ float lds[256 * 16 * M];
+    __shared__ float lds_db[256 * M];
+    const int t = threadIdx.x;
+    const int p0 = blockIdx.y * kThinPieces, all = a.kp / 16;
+    const int pieces = all - p0 < kThinPieces ? all - p0 : kThinPieces, lanes = 256 / pieces;  // rows side by side
+    const int c = t % pieces, rl = t / pieces;
+    const int64_t lo = blockIdx.x * a.rows_per;
+    const int64_t hi = lo + a.rows_per < a.n ? lo + a.rows_per : a.n;
+    float acc[M][16], db[M];
+#pragma unroll
+    for (int j = 0; j < M; ++j) {
+        db[j] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[j][i] = 0.f;
+    }
+    constexpr int U = 4;  // rows of a thread on their way at a time
+    if (rl < lanes && hi > lo) {
+        const signed char* q = a.q + (p0 + c) * 16;
+        for (int64_t row0 = lo + rl; row0 < hi; row0 += U * lanes) {
+            i32x4 x[U];
+            float s[U], d[U][M];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t row = row0 + u * lanes < hi ? row0 + u * lanes : hi - 1;
+                x[u] = *(const i32x4*)(q + row * a.kp);
+                s[u] = a.scale[row];
+#pragma unroll
+                for (int j = 0; j < M; ++j) d[u][j] = (float)((const T*)a.dz)[row * a.lddz + j];
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const bool on = row0 + u * lanes < hi;
+#pragma unroll
+                for (int j = 0; j < M; ++j) {
+                    d[u][j] = on ? d[u][j] : 0.f;
+                    db[j] += d[u][j];
+                    d[u][j] *= on ? s[u] : 0.f;
+                }
+#pragma unroll
+                for (int w = 0; w < 4; ++w)
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        const float v = (float)((x[u][w] << (24 - 8 * b)) >> 24);
+#pragma unroll
+                        for (int j = 0; j < M; ++j) acc[j][4 * w + b] = __builtin_fmaf(v, d[u][j], acc[j][4 * w + b]);
+                    }
+            }
+        }
+    }
+    if (rl < lanes) {
+#pragma unroll
+        for (int j = 0; j < M; ++j) {
+            if (c == 0) lds_db[rl * M + j] = db[j];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) lds[((rl * pieces + c) * 16 + i) * M + j] = acc[j][i];
+        }
+    }
+    __syncthreads();
+    for (int e = t; e < pieces * 16 * M; e += 256) {
+        float s = 0.f;
+        for (int r = 0; r < lanes; ++r) s += lds[r * pieces * 16 * M + e];
+        const int f = p0 * 16 + e / M;
+        if (f < a.k) a.out[blockIdx.x * a.stride + (size_t)f * M + e % M] = s;
+    }
+    if (blockIdx.y == 0 && t < M) {
+        float s = 0.f;
+        for (int r = 0; r < lanes; ++r) s += lds_db[r * M + t];
+        a.out_db[blockIdx.x * a.stride + t] = s;
     }
 }
 
@@ -244,24 +341,53 @@ __global__ __launch_bounds__(256) void grad_weight_join_kernel(const float* __re
     }
 }
 
-// How the rows are cut: enough slices for two workgroups per CU over all tiles, none under 256 rows.
+// Which tiles, and how the rows are cut: up to `target` workgroups over all tiles, slices of at least 256 rows.
 struct Cut {
-    int kblocks, mblocks, tile_m, slices;
+    int tile_k, tile_m;  // tile_m 0: the kernel for few outputs
+    int kblocks, mblocks, slices;
     int64_t rows_per;
 };
 static Cut cut_rows(int64_t n, int k, int m) {
     Cut c;
-    c.tile_m = m <= 32 ? 32 : 128;
-    c.kblocks = (k + kTileK - 1) / kTileK, c.mblocks = (m + c.tile_m - 1) / c.tile_m;
+    const bool thin = m <= 4;
+    c.tile_m = thin ? 0 : m <= 32 ? 32 : 128;
+    c.tile_k = thin ? kThinPieces * 16 : (m > 32 && k <= 64) ? 64 : 128;
+    c.kblocks = (k + c.tile_k - 1) / c.tile_k, c.mblocks = thin ? 1 : (m + c.tile_m - 1) / c.tile_m;
     const int64_t blocks = (int64_t)c.kblocks * c.mblocks;
-    int64_t s = 512 / blocks;
+    const int64_t target = c.tile_m == 128 ? 512 : 1024;  // two or more workgroups a CU, as their registers allow
+    int64_t s = target / blocks;
     const int64_t most = (n + 255) / 256;
     if (s > most) s = most;
     if (s >= 8) s = s / 8 * 8;
     if (s < 1) s = 1;
     c.slices = (int)s;
-    c.rows_per = ((n + s - 1) / s + kStageRows - 1) / kStageRows * kStageRows;
+    c.rows_per = ((n + s - 1) / s + 63) / 64 * 64;
     return c;
+}
+
+template <int DT>
+static void launch_grad_weight(const GradWeightArgs& a, const Cut& c, hipStream_t st) {
+    if (c.tile_m == 0) {
+        const dim3 grid(c.slices, c.kblocks);
+        if (a.m == 1) grad_weight_thin_kernel<DT, 1><<<grid, 256, 0, st>>>(a);
+        else if (a.m == 2) grad_weight_thin_kernel<DT, 2><<<grid, 256, 0, st>>>(a);
+        else if (a.m == 3) grad_weight_thin_kernel<DT, 3><<<grid, 256, 0, st>>>(a);
+        else grad_weight_thin_kernel<DT, 4><<<grid, 256, 0, st>>>(a);
+        return;
+    }
+    const unsigned grid = (unsigned)((int64_t)c.kblocks * c.mblocks * c.slices);
+    constexpr int D = DT == NERF_F32 ? 2 : 4;
+    const bool even = a.m % 8 == 0;
+    if (c.tile_m == 32) grad_weight_kernel<DT, 128, 32, 32, 4, false><<<grid, 256, 0, st>>>(a);
+    else if (c.tile_k == 64) {
+        if (even) grad_weight_kernel<DT, 64, 128, 32, D, true><<<grid, 256, 0, st>>>(a);
+        else grad_weight_kernel<DT, 64, 128, 32, D, false><<<grid, 256, 0, st>>>(a);
+    } else {
+        // (stages of 64 rows where LDS holds two of them twice over: 786432 x 256 x 256, 198 -> 182 us)
+        if (even && DT == NERF_BF16) grad_weight_kernel<DT, 128, 128, DT == NERF_BF16 ? 64 : 32, 2, true><<<grid, 256, 0, st>>>(a);
+        else if (even) grad_weight_kernel<DT, 128, 128, 32, D, true><<<grid, 256, 0, st>>>(a);
+        else grad_weight_kernel<DT, 128, 128, 32, D, false><<<grid, 256, 0, st>>>(a);
+    }
 }
 
 }  // namespace i8
@@ -296,18 +422,10 @@ NERF_API int nerf_linear_int8_grad_weight(const signed char* q, const float* sca
     const size_t n_dw = (size_t)k * m;
     if (c.slices > 1) a.out = (float*)workspace, a.out_db = (float*)workspace + n_dw, a.stride = n_dw + m;
     else a.out = dw, a.out_db = db, a.stride = 0;
-    const unsigned grid = (unsigned)((int64_t)c.kblocks * c.mblocks * c.slices);
     hipStream_t st = as_stream(stream);
-#define NERF_W(DT)                                                                     \
-    do {                                                                               \
-        if (c.tile_m == 32) grad_weight_kernel<DT, 32, false><<<grid, 256, 0, st>>>(a);     \
-        else if (m % 8 == 0) grad_weight_kernel<DT, 128, true><<<grid, 256, 0, st>>>(a);    \
-        else grad_weight_kernel<DT, 128, false><<<grid, 256, 0, st>>>(a);                   \
-    } while (0)
-    if (dtype == NERF_F32) NERF_W(NERF_F32);
-    else if (dtype == NERF_F16) NERF_W(NERF_F16);
-    else NERF_W(NERF_BF16);
-#undef NERF_W
+    if (dtype == NERF_F32) launch_grad_weight<NERF_F32>(a, c, st);
+    else if (dtype == NERF_F16) launch_grad_weight<NERF_F16>(a, c, st);
+    else launch_grad_weight<NERF_BF16>(a, c, st);
     if (int rc = check_launch(what)) return rc;
     if (c.slices > 1) {
         grad_weight_join_kernel<<<(unsigned)((n_dw + m + 31) / 32), 256, 0, st>>>((const float*)workspace, c.slices, a.stride, n_dw, n_dw + m, dw, db);
