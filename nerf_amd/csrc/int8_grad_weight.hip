@@ -92,25 +92,41 @@ __global__ __launch_bounds__(256, 2) void grad_weight_kernel(GradWeightArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum[i][j] = 0.f;
 
-    // rows from row0; those behind `most` repeat it
-    auto fetch = [&](int64_t row0, int64_t most, Held& h) {
+    // Where a thread's pieces are, from the first row of a stage: the same for every stage, so that a fetch is a
+    // scalar base and these.
+    unsigned x_at[CX], s_at[CX];
+    int64_t y_at[CY];
+#pragma unroll
+    for (int i = 0; i < CX; ++i) {
+        const int e = t + 256 * i, col = kb * KT + x_img(e) * 32 + x_half(e) * 16;
+        x_at[i] = (unsigned)x_row(e) * a.kp + (col < a.kp ? col : 0);  // (behind the last column: not stored)
+        s_at[i] = x_row(e);
+    }
+    auto y_col = [&](int i) {
+        const int col = mb * MT + y_img(t + 256 * i) * 32 + yq * 8;
+        return EVEN && col >= a.m ? 0 : col;
+    };
+#pragma unroll
+    for (int i = 0; i < CY; ++i) y_at[i] = y_row(t + 256 * i) * a.lddz;
+    // the stage from row0, which has rows at least up to row0 + `most`; rows behind repeat that one
+    auto fetch = [&](int64_t row0, int most, Held& h) {
         if (has_x) {
+            const signed char* q = a.q + row0 * a.kp;
+            const float* sc = a.scale + row0;
 #pragma unroll
             for (int i = 0; i < CX; ++i) {
-                const int e = t + 256 * i, col = kb * KT + x_img(e) * 32 + x_half(e) * 16;
-                const int64_t row = row0 + x_row(e) < most ? row0 + x_row(e) : most;
-                h.x[i] = *(const i32x4*)(a.q + row * a.kp + (col < a.kp ? col : 0));  // (behind the last: not stored)
-                h.s[i] = a.scale[row];
+                const unsigned back = (int)s_at[i] > most ? s_at[i] - most : 0u;
+                h.x[i] = *(const i32x4*)(q + (x_at[i] - back * a.kp));
+                h.s[i] = sc[s_at[i] - back];
             }
         }
         if (has_y) {
+            const T* y = (const T*)a.dz + row0 * a.lddz;
 #pragma unroll
             for (int i = 0; i < CY; ++i) {
-                const int e = t + 256 * i, col = mb * MT + y_img(e) * 32 + yq * 8;
-                const int64_t row = row0 + y_row(e) < most ? row0 + y_row(e) : most;
-                const T* src = (const T*)a.dz + row * a.lddz;
-                if constexpr (EVEN) h.y[i] = load8<T>(src, col < a.m ? col : 0, a.m, true);
-                else h.y[i] = load8<T>(src, col, a.m, y_whole);
+                const int row = y_row(t + 256 * i);
+                const T* src = y + (y_at[i] - (row > most ? (row - most) * a.lddz : 0));
+                h.y[i] = load8<T>(src, y_col(i), a.m, EVEN || y_whole);
             }
         }
     };
@@ -162,48 +178,63 @@ __global__ __launch_bounds__(256, 2) void grad_weight_kernel(GradWeightArgs a) {
         for (int y = 0; y < AY; ++y)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
+    // 16 rows at a time; the operands of the next 16 are read before the products of these (left to itself the
+    // compiler reads right before use, and every product waits for LDS)
+    struct Operands {
+        bf16x8 x[AX], y[N][AY];
+    };
+    auto read = [&](const char* buf, int half, Operands& o) {
+#pragma unroll
+        for (int x = 0; x < AX; ++x) o.x[x] = tr_operand(buf + (wx + x) * kImg, half, lane);
+#pragma unroll
+        for (int s = 0; s < N; ++s)
+#pragma unroll
+            for (int y = 0; y < AY; ++y) o.y[s][y] = tr_operand(buf + (XT + s * YT + wy + y) * kImg, half, lane);
+    };
     auto multiply = [&](const char* buf) {
+        Operands o[2];
+        read(buf, 0, o[0]);
 #pragma unroll
         for (int half = 0; half < R / 16; ++half) {
-            bf16x8 xo[AX];
-#pragma unroll
-            for (int x = 0; x < AX; ++x) xo[x] = tr_operand(buf + (wx + x) * kImg, half, lane);
+            if (half + 1 < R / 16) read(buf, half + 1, o[(half + 1) & 1]);
+            __builtin_amdgcn_sched_barrier(0);
+            const Operands& c = o[half & 1];
 #pragma unroll
             for (int s = 0; s < N; ++s)
 #pragma unroll
-                for (int y = 0; y < AY; ++y) {
-                    const bf16x8 yo = tr_operand(buf + (XT + s * YT + wy + y) * kImg, half, lane);
+                for (int y = 0; y < AY; ++y)
 #pragma unroll
-                    for (int x = 0; x < AX; ++x) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xo[x], yo, acc[x][y], 0, 0, 0);
-                }
+                    for (int x = 0; x < AX; ++x) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(c.x[x], c.y[s][y], acc[x][y], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // every fetch is made, also of stages that do not exist (they repeat the last row): a wait for older
-    // loads counts the younger ones
-    if (hi > lo) {
+    // every fetch is made, also of stages that do not exist (they repeat the last): a wait for older loads
+    // counts the younger ones
+    if (stages > 0) {
+        auto fetch_whole = [&](int64_t st, Held& h) { fetch(lo + (st < stages ? st : stages - 1) * R, R - 1, h); };
 #pragma unroll
-        for (int d = 0; d < D; ++d) fetch(lo + d * R, hi - 1, held[d]);
-        if (stages > 0) stage(held[0], lds, R);
+        for (int d = 0; d < D; ++d) fetch_whole(d, held[d]);
+        stage(held[0], lds, R);
         __syncthreads();
         for (int64_t st0 = 0; st0 < stages; st0 += D) {
 #pragma unroll
             for (int d = 0; d < D; ++d) {
                 const int64_t st = st0 + d;
                 if (st >= stages) break;
-                fetch(lo + (st + D) * R, hi - 1, held[d]);
+                fetch_whole(st + D, held[d]);
                 multiply(lds + (d & 1) * kStage);
                 // into the buffer that was read in the turn before this one
                 if (st + 1 < stages) stage(held[(d + 1) % D], lds + ((d + 1) & 1) * kStage, R);
                 __syncthreads();
             }
         }
-        if (left > 0) {
-            fetch(lo + stages * R, hi - 1, held[0]);
-            stage(held[0], lds, left);
-            __syncthreads();
-            multiply(lds);
-            __syncthreads();
-        }
+    }
+    if (left > 0) {
+        fetch(lo + stages * R, left - 1, held[0]);
+        stage(held[0], lds, left);
+        __syncthreads();
+        multiply(lds);
+        __syncthreads();
     }
 
     float* out = a.out + slice * a.stride;
