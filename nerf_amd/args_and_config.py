@@ -50,6 +50,8 @@ OPTIONS = [
     ("autoencoded_keypoints_filename", str, None), ("learnable_embeddings_filename", str, None),
     ("trainskip", int, 1), ("depth_from_camera", _FLAG, False), ("test_finish", int, None),
     ("near", float, None), ("far", float, None), ("frames_field", str, 'frames'), ("depth_loss", _FLAG, False),
+    # not in the reference: 'int8' trains and queries networks of any depth and width on the 8-bit layers
+    ("precision", str, None),
 ]
 _BY_NAME = {name: (typ, default) for name, typ, default in OPTIONS}
 

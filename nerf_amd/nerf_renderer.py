@@ -10,6 +10,7 @@ resampling+merge, fused encoding+MLP, compositing.
 import torch
 
 from . import _native as nv
+from . import layered
 from . import ops
 from . import training
 from .run_nerf_helpers import NerfModel
@@ -18,9 +19,14 @@ from .run_nerf_helpers import NerfModel
 SINGLE_CALL = True  # inference through nerf_render_rays (one C-ABI call per chunk) when nothing else is asked for
 
 
-def _check_embedders(embed_fn, embeddirs_fn):
+def _check_embedders(embed_fn, embeddirs_fn, fn):
     m = getattr(embed_fn, 'multires', None)
     mv = getattr(embeddirs_fn, 'multires', None)
+    if fn.layered:
+        if 3 + 6 * (m or 0) != fn.input_ch or 3 + 6 * (mv or 0) != fn.input_ch_views:
+            raise ValueError(f"run_network: encoders of {m} and {mv} octaves for a network of {fn.input_ch} and "
+                             f"{fn.input_ch_views} inputs")
+        return
     if m != 10 or mv != 4:
         raise NotImplementedError(
             "the fused MLP kernel encodes points with multires=10 and view directions with "
@@ -35,13 +41,17 @@ def run_network(inputs, viewdirs, fn, embed_fn, embeddirs_fn, netchunk=1024 * 64
         raise TypeError("run_network: network_fn must come from init_nerf_model")
     if viewdirs is None:
         raise NotImplementedError("run_network: the built network takes view directions (use_viewdirs=True)")
-    _check_embedders(embed_fn, embeddirs_fn)
+    _check_embedders(embed_fn, embeddirs_fn, fn)
     pts = nv.f32(inputs)
     lead = tuple(pts.shape[:-1])
     if pts.dim() == 2:
         pts = pts[:, None, :]
     pts = pts.reshape(pts.shape[0], -1, 3)
     vd = nv.f32(viewdirs, pts.device).reshape(-1, 3)
+    if fn.layered:
+        if vd.shape[0] != pts.shape[0]:
+            raise ValueError(f"run_network: {pts.shape[0]} rays of points and {vd.shape[0]} view directions")
+        return layered.query(fn, pts.reshape(-1, 3), vd, pts.shape[1]).reshape(lead + (4,))
     raw = ops.mlp_forward_pts(fn.packed(), pts, vd)
     return raw.reshape(lead + (4,))
 
@@ -92,7 +102,8 @@ def render_rays(ray_batch, network_fn, network_query_fn, N_samples, retraw=False
     # timers are armed.
     if (SINGLE_CALL and fused and not rec and not retraw and not raw_noise_std > 0. and n > 0
             and ops.MLP_TIMING is None and ops.HBM_TIMING is None
-            and isinstance(network_fn, NerfModel) and (network_fine is None or isinstance(network_fine, NerfModel))):
+            and isinstance(network_fn, NerfModel) and (network_fine is None or isinstance(network_fine, NerfModel))
+            and not network_fn.layered and not (network_fine is not None and network_fine.layered)):
         if N_importance > 0 and perturb > 0.:
             if pdf_u is None:
                 pdf_u = torch.rand((n, N_importance), dtype=torch.float32, device=rays.device)
@@ -105,9 +116,12 @@ def render_rays(ray_batch, network_fn, network_query_fn, N_samples, retraw=False
                                            rays, N_samples, N_importance, lindisp, white_bkgd, perturb_u, pdf_u)
 
     def query(z, net):
+        by_layer = getattr(net, 'layered', False)
+        if rec and by_layer:
+            return layered.LayeredQuery.apply(rays, z, net, *net.params)
         if rec:
             return training.MLPQuery.apply(rays, z, net, *net.params)
-        if fused:
+        if fused and not by_layer:
             return ops.mlp_forward_rays(net.packed(), rays, z)
         pts = rays[:, None, 0:3] + rays[:, None, 3:6] * z[:, :, None]
         return nv.f32(network_query_fn(pts, rays[:, 8:11], net), rays.device)

@@ -525,9 +525,10 @@ def quantize_rows(x, pow2=False, want_mask=False):
     return Int8Rows._made(q, scale, k, pow2, mask)
 
 
-def pack_int8(w, pow2=False):
+def pack_int8(w, pow2=False, into=None):
     """Int8Weights of a kernel W [k, m] (fp32, [in, out]): one scale per output channel.  pow2 also lays out
-    what linear_int8_grad_input reads."""
+    what linear_int8_grad_input reads.  into: Int8Weights of the same shape and kind whose memory is
+    overwritten (behind the work that the current stream has queued)."""
     dev = _on_gpu("pack_int8", w)
     if w.dim() != 2 or w.shape[0] < 1 or w.shape[1] < 1:
         raise ValueError(f"pack_int8: expected [k >= 1, m >= 1], got {tuple(w.shape)}")
@@ -536,9 +537,14 @@ def pack_int8(w, pow2=False):
     need = int(nv.lib().nerf_int8_packed_bytes(k, m, int(bool(pow2))))
     if need == 0:
         raise ValueError(f"pack_int8: widths {k} x {m} are beyond what the kernels are built for")
-    packed = torch.empty((need,), dtype=torch.uint8, device=dev)
+    if into is None:
+        packed = torch.empty((need,), dtype=torch.uint8, device=dev)
+    elif not isinstance(into, Int8Weights) or (into.k, into.m, into.pow2, into.packed.device) != (k, m, bool(pow2), dev):
+        raise ValueError(f"pack_int8: into={into!r} does not hold {k} x {m} weights, pow2={bool(pow2)}, on {dev}")
+    else:
+        packed = into.packed
     _call("nerf_int8_pack", dev, w.data_ptr(), k, m, 1 if pow2 else 0, packed.data_ptr())
-    return Int8Weights(packed, k, m, bool(pow2))
+    return Int8Weights(packed, k, m, bool(pow2)) if into is None else into
 
 
 def _linear_inputs(what, rows, weights, bias, addend):

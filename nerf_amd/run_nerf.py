@@ -125,9 +125,10 @@ def create_nerf(args):
     if getattr(args, 'keypoint_embedding_size', None):
         raise NotImplementedError("keypoint networks (NERFCO.nerf_keypoint_network, run_nerf.py:186-195) "
                                   "are not part of this build")
+    precision = getattr(args, 'precision', None)  # 'int8': networks of any depth and width, layer by layer
     model = init_nerf_model(D=args.netdepth, W=args.netwidth, input_ch=input_ch, output_ch=output_ch,
                             skips=skips, input_ch_views=input_ch_views,
-                            use_viewdirs=args.use_viewdirs)                            # :176-179
+                            use_viewdirs=args.use_viewdirs, precision=precision)       # :176-179
     grad_vars = model.trainable_variables
     models = {'model': model}
     model_fine = None
@@ -135,7 +136,7 @@ def create_nerf(args):
         model_fine = init_nerf_model(D=args.netdepth_fine, W=args.netwidth_fine, input_ch=input_ch,
                                      output_ch=output_ch, skips=skips,
                                      input_ch_views=input_ch_views,
-                                     use_viewdirs=args.use_viewdirs)                   # :197-201
+                                     use_viewdirs=args.use_viewdirs, precision=precision)  # :197-201
         grad_vars = grad_vars + model_fine.trainable_variables                         # :206
         models['model_fine'] = model_fine
 

@@ -85,8 +85,10 @@ class NerfModel:
     Parameter order (get_weights()): kernel [in,out], bias [out] of the D point layers, then
     bottleneck, view layer, rgb, alpha."""
 
-    def __init__(self, D, W, input_ch, input_ch_views, output_ch, skips, use_viewdirs, device=None,
-                 generator=None):
+    layered = False   # whether it is evaluated layer by layer (nerf_amd.layered) instead of by the fused kernels
+
+    @staticmethod
+    def check_shape(D, W, input_ch, input_ch_views, output_ch, skips, use_viewdirs):
         if not (D == 8 and W == 256 and input_ch == 63 and input_ch_views == 27
                 and tuple(skips) == (4,) and use_viewdirs and output_ch == 4):
             raise NotImplementedError(
@@ -94,6 +96,10 @@ class NerfModel:
                 "D=8, W=256, input_ch=63 (multires=10), input_ch_views=27 (multires_views=4), "
                 f"skips=[4], use_viewdirs=True; got D={D} W={W} input_ch={input_ch} "
                 f"input_ch_views={input_ch_views} skips={list(skips)} use_viewdirs={use_viewdirs}")
+
+    def __init__(self, D, W, input_ch, input_ch_views, output_ch, skips, use_viewdirs, device=None,
+                 generator=None):
+        self.check_shape(D, W, input_ch, input_ch_views, output_ch, skips, use_viewdirs)
         self.D, self.W, self.input_ch, self.input_ch_views = D, W, input_ch, input_ch_views
         self.skips, self.use_viewdirs = tuple(skips), use_viewdirs
         dev = ops._dev() if device is None else torch.device(device)
@@ -123,7 +129,7 @@ class NerfModel:
             at += fo
             self.params.append(w.requires_grad_(True))
             self.params.append(bvec.requires_grad_(True))
-        self._packed = torch.empty((ops.packed_bytes(),), dtype=torch.uint8, device=dev) if dev.type == 'cuda' else None
+        self._packed = torch.empty((ops.packed_bytes(),), dtype=torch.uint8, device=dev) if dev.type == 'cuda' and not self.layered else None
         self._packed_bwd = None
         self._packed_version = None
         self._packed_bwd_version = None
@@ -176,6 +182,8 @@ class NerfModel:
 
     def packed(self):
         """The fp16 fragment stream for the current parameter values (re-packed when they change)."""
+        if self.layered:
+            raise NotImplementedError("a layered network has no fused weight stream")
         ver = self._version()
         if ver != self._packed_version:
             with torch.no_grad():
@@ -243,10 +251,17 @@ class NerfModel:
 
 
 def init_nerf_model(D=8, W=256, input_ch=3, input_ch_views=3, output_ch=4, skips=[4],
-                    use_viewdirs=False, device=None, generator=None):
-    """run_nerf_helpers.py:80-117."""
-    return NerfModel(int(D), int(W), int(input_ch), int(input_ch_views), int(output_ch), list(skips),
-                     bool(use_viewdirs), device=device, generator=generator)
+                    use_viewdirs=False, device=None, generator=None, precision=None):
+    """run_nerf_helpers.py:80-117.  precision (not in the reference): None for the fused fp16 network of the
+    configured shape, 'int8' for one of any depth and width on the 8-bit layers (nerf_amd.layered)."""
+    if precision is None:
+        cls = NerfModel
+    elif precision == 'int8':
+        from .layered import LayeredNerfModel as cls
+    else:
+        raise ValueError(f"init_nerf_model: precision must be None or 'int8', got {precision!r}")
+    return cls(int(D), int(W), int(input_ch), int(input_ch_views), int(output_ch), list(skips),
+               bool(use_viewdirs), device=device, generator=generator)
 
 
 # ---- rays (run_nerf_helpers.py:122-180) --------------------------------------------------------
