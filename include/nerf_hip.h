@@ -315,14 +315,15 @@ int nerf_int8_pack(const float* w, int k, int m, int pow2, void* packed, nerf_st
 /* y [n][m] = ((sum_f q[i][f] p[f][j]) * channel scale j) * row scale i (+ bias[j]) (+ addend[i][j]), then
  * relu when asked; the integer sums are exact; in fp32 are rounded: the sum, its product with the
  * channel scale, that times the row scale plus the bias (once), the addition of the addend; the result
- * to y's type.  bias [m] or NULL; addend: [n][m] of any of the three types or NULL; y must not overlap an
+ * to y's type.  bias [m] or NULL; addend: [n][m] fp32 or bf16, or NULL; y must not overlap an
  * input. */
 int nerf_linear_int8(const signed char* q, const float* scale, int64_t n, int k, const void* packed, int m,
                      const float* bias, const void* addend, int addend_dtype, int64_t ldadd, int relu,
                      void* y, int dtype, int64_t ldy, nerf_stream_t stream);
 
 /* nerf_quantize_rows of that y (in fp32, never stored): the next layer's rows, yq [n][m rounded up to 64].  For
- * m up to nerf_linear_int8_quantized_width(k) (256 for k up to 576, else 0); wider: NERF_E_UNSUPPORTED. */
+ * m up to nerf_linear_int8_quantized_width(k) (256 for k up to 576, else 0), and with an addend m a
+ * multiple of 64; otherwise NERF_E_UNSUPPORTED. */
 int nerf_linear_int8_quantized_width(int k);
 int nerf_linear_int8_quantized(const signed char* q, const float* scale, int64_t n, int k, const void* packed, int m,
                                const float* bias, const void* addend, int addend_dtype, int64_t ldadd, int relu,

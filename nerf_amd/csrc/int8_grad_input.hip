@@ -11,9 +11,9 @@ template <int DT> constexpr int kHeld = DT == NERF_F32 ? 4 : 8;
 
 template <int DT, int NT>
 static int resident(const LinearArgs& a, const char* what, hipStream_t st) {
-    if (a.width % 32 != 0) return launch_resident<Bf16Op<DT, false>, DT, NT, 2, 1, false>(a, what, st);
-    if (a.steps <= 2) return launch_resident<Bf16Op<DT, true>, DT, NT, 2, 1, false>(a, what, st);
-    return launch_resident<Bf16Op<DT, true>, DT, NT, kHeld<DT>, 1, false>(a, what, st);
+    if (a.width % 32 != 0) return launch_resident<Bf16Op<DT, false>, DT, NT, 2, 1, NO_ADD>(a, what, st);
+    if (a.steps <= 2) return launch_resident<Bf16Op<DT, true>, DT, NT, 2, 1, NO_ADD>(a, what, st);
+    return launch_resident<Bf16Op<DT, true>, DT, NT, kHeld<DT>, 1, NO_ADD>(a, what, st);
 }
 
 template <int DT>
@@ -21,9 +21,9 @@ static int launch(const LinearArgs& a, const char* what, hipStream_t st) {
     const int nt = resident_groups(a);
     if constexpr (DT == NERF_BF16) {
         if (a.n >= kResidentRows && (nt == 0 || a.groups > nt) && a.width % 32 == 0 && a.lddz % 8 == 0 && ((uintptr_t)a.dz & 15) == 0)
-            return launch_streamed<Bf16Op<DT, true>, DT, false>(a, what, st);
+            return launch_streamed<Bf16Op<DT, true>, DT, NO_ADD>(a, what, st);
     }
-    if (a.n < kResidentRows || nt == 0) return launch_direct<Bf16Op<DT, false>, DT, false>(a, what, st);
+    if (a.n < kResidentRows || nt == 0) return launch_direct<Bf16Op<DT, false>, DT, NO_ADD>(a, what, st);
     if (nt == 4) return resident<DT, 4>(a, what, st);
     if (nt == 2) return resident<DT, 2>(a, what, st);
     return resident<DT, 1>(a, what, st);

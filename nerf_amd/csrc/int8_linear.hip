@@ -9,11 +9,14 @@ constexpr int64_t kResidentRows = 4096;
 
 // Tiles of 16 points a wave works on at a time: two halve the reads of LDS and of the channel scales, where
 // the registers hold the sums of both.
-template <int OUT, int NT, int CH, bool ADD> constexpr int kTiles = (NT == 4 && (CH > 4 || ADD || OUT >= TO_INT8)) || (NT == 2 && ADD && OUT >= TO_INT8) ? 1 : 2;
+template <int OUT, int NT, int CH, int ADD>
+constexpr int kTiles = (NT == 4 && (CH > 4 || ADD != NO_ADD || OUT >= TO_INT8)) || (NT == 2 && ADD != NO_ADD && OUT >= TO_INT8) ? 1 : 2;
 
-template <int OUT, int NT, bool ADD>
+template <int OUT, int NT, int ADD>
 static int resident(const LinearArgs& a, const char* what, hipStream_t st) {
-    switch (a.steps) {  // all of a row in one unit up to 320 inputs
+    // all of a row in one unit up to 320 inputs (beside an addend's memory traffic a step read twice costs little)
+    if constexpr (ADD != NO_ADD) return launch_resident<Int8Op, OUT, NT, 4, kTiles<OUT, NT, 4, ADD>, ADD>(a, what, st);
+    else switch (a.steps) {
         case 1: return launch_resident<Int8Op, OUT, NT, 1, kTiles<OUT, NT, 1, ADD>, ADD>(a, what, st);
         case 2: return launch_resident<Int8Op, OUT, NT, 2, kTiles<OUT, NT, 2, ADD>, ADD>(a, what, st);
         case 5: return launch_resident<Int8Op, OUT, NT, 5, kTiles<OUT, NT, 5, ADD>, ADD>(a, what, st);
@@ -22,7 +25,7 @@ static int resident(const LinearArgs& a, const char* what, hipStream_t st) {
     }
 }
 
-template <int OUT, bool ADD>
+template <int OUT, int ADD>
 static int launch(const LinearArgs& a, const char* what, hipStream_t st) {
     const int nt = resident_groups(a);
     if constexpr (OUT < TO_INT8) {
@@ -35,15 +38,16 @@ static int launch(const LinearArgs& a, const char* what, hipStream_t st) {
 }
 
 template <int OUT>
-static int launch(const LinearArgs& a, const char* what, hipStream_t st) {
-    return a.addend ? launch<OUT, true>(a, what, st) : launch<OUT, false>(a, what, st);
+static int launch(const LinearArgs& a, int add_dtype, const char* what, hipStream_t st) {
+    if (!a.addend) return launch<OUT, NO_ADD>(a, what, st);
+    return add_dtype == NERF_F32 ? launch<OUT, NERF_F32>(a, what, st) : launch<OUT, NERF_BF16>(a, what, st);
 }
 
 // Checks and fields that both entry points share.
 static int linear_args(LinearArgs& a, const char* what, const signed char* q, const float* scale, int64_t n, int k,
                        const void* packed, int m, const float* bias, const void* addend, int addend_dtype, int64_t ldadd, int relu) {
     if (int rc = require_widths(what, n, k, m)) return rc;
-    NERF_REQUIRE(!addend || dtype_ok(addend_dtype), "%s: unknown type", what);
+    NERF_REQUIRE(!addend || addend_dtype == NERF_F32 || addend_dtype == NERF_BF16, "%s: an addend is fp32 or bf16", what);
     if (n == 0) return 0;
     NERF_REQUIRE(q && scale && packed, "%s: null pointer", what);
     NERF_REQUIRE(!addend || ldadd >= m, "%s: rows of %d elements overlap", what, m);
@@ -53,7 +57,7 @@ static int linear_args(LinearArgs& a, const char* what, const signed char* q, co
     const PackedLayout lay(k, m, false);
     a.frags = (const char*)packed + lay.frags, a.groups = lay.mp / 64, a.steps = a.frag_steps = lay.kp / 64, a.n = n;
     a.q = q, a.scale = scale, a.features = m, a.wscale = (const float*)packed, a.bias = bias;
-    a.addend = addend, a.add_dtype = addend_dtype, a.ldadd = ldadd, a.relu = relu;
+    a.addend = addend, a.ldadd = ldadd, a.relu = relu;
     return 0;
 }
 
@@ -74,9 +78,9 @@ NERF_API int nerf_linear_int8(const signed char* q, const float* scale, int64_t 
     NERF_REQUIRE(y && ldy >= m && ((uintptr_t)y & (dtype_size(dtype) - 1)) == 0, "%s: y must be aligned rows that do not overlap", what);
     a.out = y, a.ldout = ldy;
     hipStream_t st = as_stream(stream);
-    if (dtype == NERF_F32) return launch<NERF_F32>(a, what, st);
-    if (dtype == NERF_F16) return launch<NERF_F16>(a, what, st);
-    return launch<NERF_BF16>(a, what, st);
+    if (dtype == NERF_F32) return launch<NERF_F32>(a, addend_dtype, what, st);
+    if (dtype == NERF_F16) return launch<NERF_F16>(a, addend_dtype, what, st);
+    return launch<NERF_BF16>(a, addend_dtype, what, st);
 }
 
 NERF_API int nerf_linear_int8_quantized_width(int k) {
@@ -92,11 +96,13 @@ NERF_API int nerf_linear_int8_quantized(const signed char* q, const float* scale
     if (int rc = linear_args(a, what, q, scale, n, k, packed, m, bias, addend, addend_dtype, ldadd, relu)) return rc;
     if (m > nerf_linear_int8_quantized_width(k))
         return NERF_FAIL(NERF_E_UNSUPPORTED, "%s: %d inputs and %d outputs do not fit one workgroup", what, k, m);
+    if (addend && m % 64 != 0)
+        return NERF_FAIL(NERF_E_UNSUPPORTED, "%s: an addend of %d columns is not a whole number of 64", what, m);
     if (n == 0) return 0;
     NERF_REQUIRE(yq && yscale, "%s: null pointer", what);
     NERF_REQUIRE(((uintptr_t)yq & 15) == 0 && ((uintptr_t)yscale & 3) == 0 && ((uintptr_t)ymask & 1) == 0, "%s: misaligned pointer", what);
     a.out = yq, a.out_scale = yscale, a.out_mask = ymask;
     hipStream_t st = as_stream(stream);
-    if (pow2) return relu ? launch<TO_INT8 + 3>(a, what, st) : launch<TO_INT8 + 2>(a, what, st);
-    return relu ? launch<TO_INT8 + 1>(a, what, st) : launch<TO_INT8>(a, what, st);
+    if (pow2) return relu ? launch<TO_INT8 + 3>(a, addend_dtype, what, st) : launch<TO_INT8 + 2>(a, addend_dtype, what, st);
+    return relu ? launch<TO_INT8 + 1>(a, addend_dtype, what, st) : launch<TO_INT8>(a, addend_dtype, what, st);
 }

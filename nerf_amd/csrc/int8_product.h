@@ -27,8 +27,7 @@ struct LinearArgs {
     int features;          // of a row of the output
     const float* wscale;
     const float* bias;
-    const void* addend;    // [n][ldadd] or null
-    int add_dtype;
+    const void* addend;    // [n][ldadd] of the type the kernel is instantiated for
     int64_t ldadd;
     int relu;
     const unsigned char* mask;
@@ -42,6 +41,8 @@ struct LinearArgs {
 // What a product is stored as: a type (NERF_F32, ...) or 8-bit rows: TO_INT8, + 1 behind a ReLU, + 2 with
 // scales that are powers of two.
 constexpr int TO_INT8 = 4;
+// Type of an addend: NERF_F32 or NERF_BF16 (fp16 is exact in fp32), or none.
+constexpr int NO_ADD = -1;
 
 // ---- the two products -----------------------------------------------------------------------------
 // Raw: what a lane loads of a point's row for one step; B: the operands made of it.
@@ -114,7 +115,7 @@ DEV float positive_nan(float v) { return v != v ? __builtin_bit_cast(float, 0x7f
 // y = relu((sum x channel scale) x row scale + bias + addend): the sum rounded to fp32, its product with
 // the channel scale rounded, then one rounding for row scale and bias and one for the addend.  ws, b: the
 // 16 channels' scales and biases (0 and 0 behind the last channel; a NaN without its sign).
-template <bool ADD>
+template <int ADD>
 DEV void finish_linear(const LinearArgs& a, const i32x4 (&acc)[4], const float* ws, const float* b, float xs, int f, int64_t p,
                        bool whole, bool relu, float (&v)[16]) {
 #pragma unroll
@@ -123,10 +124,9 @@ DEV void finish_linear(const LinearArgs& a, const i32x4 (&acc)[4], const float* 
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[4 * u + r] = __builtin_fmaf((float)acc[u][r] * w4[r], xs, b4[r]);
     }
-    if constexpr (ADD) {
-        if (a.add_dtype == NERF_F32) add16((const float*)a.addend + p * a.ldadd, f, a.features, whole, v);
-        else if (a.add_dtype == NERF_F16) add16((const _Float16*)a.addend + p * a.ldadd, f, a.features, whole, v);
-        else add16((const __bf16*)a.addend + p * a.ldadd, f, a.features, whole, v);
+    if constexpr (ADD != NO_ADD) {
+        typedef typename Elem<ADD>::T A;
+        add16((const A*)a.addend + p * a.ldadd, f, a.features, whole, v);
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = positive_nan(v[i]);
     }
@@ -204,7 +204,7 @@ DEV void stage_channels(const LinearArgs& a, float* ws, float* b, int f0, int co
 // ---- kernels --------------------------------------------------------------------------------------------
 
 // Few rows: one wave per group of 64 features x 32 points, operands straight from global memory.
-template <class Op, int DT, bool ADD>
+template <class Op, int DT, int ADD>
 __global__ __launch_bounds__(256) void linear_direct_kernel(LinearArgs a) {
     constexpr int P = 2;
     __shared__ __attribute__((aligned(16))) float ch[4][2][64];
@@ -272,7 +272,7 @@ constexpr int kResidentThreads = 512;
 template <int NT>
 constexpr int channel_bytes() { return 2 * NT * 64 * 4; }
 
-template <class Op, int OUT, int NT, int CH, int P, bool ADD>
+template <class Op, int OUT, int NT, int CH, int P, int ADD>
 __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(LinearArgs a, int64_t tiles) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float* const ws = (float*)lds;
@@ -331,7 +331,7 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
     auto multiply = [&](int s0, const typename Op::Raw (&from)[CH][P]) {
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
-            if (s0 + i < a.steps) {
+            if (i == 0 || s0 + i < a.steps) {  // a unit has at least one step
                 const char* w = wl + (s0 + i) * (NT * 4096) + lane * 16;
                 if constexpr (P == 1) {
                     const typename Op::B b(from[i][0]);
@@ -386,8 +386,13 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
                 unsigned top = 0u;
 #pragma unroll
                 for (int T = 0; T < NT; ++T) {
-                    finish_linear<ADD>(a, acc[j][T], ws + 64 * T + 16 * g, bs + 64 * T + 16 * g, now.xs, 64 * T + 16 * g, p,
-                                       64 * T + 64 <= a.features, RELU, v[T]);
+                    if (T < a.groups) {  // (an addend's rows are whole groups here)
+                        finish_linear<ADD>(a, acc[j][T], ws + 64 * T + 16 * g, bs + 64 * T + 16 * g, now.xs, 64 * T + 16 * g, p, true,
+                                           RELU, v[T]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[T][i] = 0.f;
+                    }
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const unsigned m = RELU ? __builtin_bit_cast(unsigned, v[T][i]) : magnitude(v[T][i]);
@@ -458,7 +463,7 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
 // then holds.
 constexpr int kStreamThreads = 512, kStreamStages = 4, kStreamStage = 32 * 1024;
 
-template <class Op, int OUT, bool ADD>
+template <class Op, int OUT, int ADD>
 __global__ __launch_bounds__(kStreamThreads) void linear_streamed_kernel(LinearArgs a, int fblocks, int64_t pblocks) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float* const ws = (float*)lds;
@@ -557,7 +562,7 @@ __global__ __launch_bounds__(kStreamThreads) void linear_streamed_kernel(LinearA
 
 constexpr int kLdsBytes = 160 * 1024;
 
-template <class Op, int OUT, int NT, int CH, int P, bool ADD>
+template <class Op, int OUT, int NT, int CH, int P, int ADD>
 int launch_resident(const LinearArgs& a, const char* what, hipStream_t st) {
     const size_t lds = channel_bytes<NT>() + (size_t)NT * a.steps * 4096;
     auto kernel = linear_resident_kernel<Op, OUT, NT, CH, P, ADD>;
@@ -575,7 +580,7 @@ int launch_resident(const LinearArgs& a, const char* what, hipStream_t st) {
     return check_launch(what);
 }
 
-template <class Op, int OUT, bool ADD>
+template <class Op, int OUT, int ADD>
 int launch_streamed(const LinearArgs& a, const char* what, hipStream_t st) {
     constexpr size_t lds = 2 * 256 * 4 + kStreamStages * kStreamStage;
     auto kernel = linear_streamed_kernel<Op, OUT, ADD>;
@@ -588,7 +593,7 @@ int launch_streamed(const LinearArgs& a, const char* what, hipStream_t st) {
     return check_launch(what);
 }
 
-template <class Op, int DT, bool ADD>
+template <class Op, int DT, int ADD>
 int launch_direct(const LinearArgs& a, const char* what, hipStream_t st) {
     const int64_t waves = (a.n + 31) / 32 * a.groups;
     if ((waves + 3) / 4 >= (1LL << 24)) return NERF_FAIL(NERF_E_UNSUPPORTED, "%s: too many rows", what);

@@ -561,6 +561,8 @@ def _linear_inputs(what, rows, weights, bias, addend):
     ldadd, add_dtype = 0, 0
     if addend is not None:
         addend, ldadd = _row_major(f"{what} (addend)", addend.detach(), weights.m)
+        if addend.dtype == torch.float16:  # exact
+            addend, ldadd = addend.float(), weights.m
         add_dtype = _DTYPES[addend.dtype]
         if addend.shape[0] != rows.n:
             raise ValueError(f"{what}: addend must have {rows.n} rows, got {addend.shape[0]}")
@@ -582,9 +584,10 @@ def linear_int8(rows, weights, bias=None, relu=False, addend=None, dtype=torch.f
 
 def linear_int8_quantized(rows, weights, bias=None, relu=False, addend=None, pow2=False, want_mask=False):
     """quantize_rows(linear_int8(...), pow2, want_mask), with y in fp32 in between: the next layer's input.  One
-    kernel that never stores y for up to 256 outputs of up to 576 inputs; the two calls otherwise."""
+    kernel that never stores y for up to 256 outputs of up to 576 inputs (with an addend a multiple of 64
+    outputs); the two calls otherwise."""
     dev, bias, addend, add_dtype, ldadd = _linear_inputs("linear_int8_quantized", rows, weights, bias, addend)
-    if weights.m > nv.lib().nerf_linear_int8_quantized_width(rows.k):
+    if weights.m > nv.lib().nerf_linear_int8_quantized_width(rows.k) or (addend is not None and weights.m % 64 != 0):
         return quantize_rows(linear_int8(rows, weights, bias, relu, addend), pow2, want_mask)
     n, m = rows.n, weights.m
     q, scale, mask = _new_rows(n, m, dev, want_mask)

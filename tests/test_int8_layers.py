@@ -52,7 +52,8 @@ def test_bad_arguments_are_refused_without_a_gpu():
                                                          ("q", "scale", "n", "k", "packed", "m", "bias", "addend", "adt", "ldadd", "relu", "pow2", "yq", "ys", "ym", "st")])
     for bad in (dict(q=None), dict(yq=None), dict(ys=None), dict(yq=odd), dict(ym=odd), dict(k=0), dict(m=0), dict(n=-1), dict(addend=one, ldadd=7)):
         assert quant(**bad) == -1, bad
-    assert quant(m=257) == -2 and quant(k=577) == -2
+    assert quant(m=257) == -2 and quant(k=577) == -2 and quant(m=65, addend=one, ldadd=65) == -2
+    assert quant(m=64, addend=one, ldadd=64, adt=1) == -1      # an addend is fp32 or bf16
     gi = lambda **c: lib.nerf_linear_int8_grad_input(*[{**dict(dz=one, dt=0, n=4, m=8, lddz=8, packed=one, k=8, mask=None, dx=one, lddx=8, st=None), **c}[x]
                                                        for x in ("dz", "dt", "n", "m", "lddz", "packed", "k", "mask", "dx", "lddx", "st")])
     for bad in (dict(dz=None), dict(dx=None), dict(packed=odd), dict(dt=3), dict(lddz=7), dict(lddx=7), dict(mask=odd), dict(k=0), dict(n=-1)):
