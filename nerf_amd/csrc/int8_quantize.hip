@@ -100,33 +100,34 @@ __global__ __launch_bounds__(kPackThreads) void int8_pack_kernel(const float* __
     __syncthreads();
     const int ksteps = lay.kp / 64, msteps = lay.mp / 32;
     const int lane = t & 63, u = (t >> 6) & 3, r = lane & 15, g = lane >> 4;
-    // integers: one 16-byte piece per thread, four steps of 64 inputs per turn of the workgroup
-    for (int s = blockIdx.y * 4 + (t >> 8); s < ksteps; s += gridDim.y * 4) {
-        const int c = frag_feature(u, r), j = 64 * T + c, f0 = 64 * s + 16 * g;
-        unsigned o[4];
+    // a step of 64 inputs per turn of the workgroup: 256 threads the integers, one 16-byte piece each, and with
+    // pow2 512 more the transposed copy in bf16 (two steps of 32 channels of this group)
+    const int part_of = t >> 8;
+    for (int s = blockIdx.y; s < ksteps; s += gridDim.y) {
+        if (part_of == 0) {
+            const int c = frag_feature(u, r), j = 64 * T + c, f0 = 64 * s + 16 * g;
+            unsigned o[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            int e[4];
+            for (int i = 0; i < 4; ++i) {
+                int e[4];
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const int f = f0 + 4 * i + b;
-                e[b] = (j < m && f < k) ? quantised(w[(size_t)f * m + j], s_inv[c]) : 0;
+                for (int b = 0; b < 4; ++b) {
+                    const int f = f0 + 4 * i + b;
+                    e[b] = (j < m && f < k) ? quantised(w[(size_t)f * m + j], s_inv[c]) : 0;
+                }
+                o[i] = pack4(e[0], e[1], e[2], e[3]);
             }
-            o[i] = pack4(e[0], e[1], e[2], e[3]);
-        }
-        *(uint4*)(packed + lay.frags + ((((size_t)T * ksteps + s) * 4 + u) * 64 + lane) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
-    }
-    if (!pow2) return;
-    // the transposed copy in bf16: two steps of 32 channels of this group for every 64 inputs
-    for (int q = blockIdx.y * 4 + (t >> 8); q < 2 * ksteps; q += gridDim.y * 4) {
-        const int tf = q >> 1, c0 = 32 * (q & 1) + 8 * g, f = 64 * tf + frag_feature(u, r);
-        bf16x8 o;
+            *(uint4*)(packed + lay.frags + ((((size_t)T * ksteps + s) * 4 + u) * 64 + lane) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+        } else if (pow2 && part_of < 3) {
+            const int half = part_of - 1, c0 = 32 * half + 8 * g, f = 64 * s + frag_feature(u, r);
+            bf16x8 o;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int j = 64 * T + c0 + i;
-            o[i] = (j < m && f < k) ? (__bf16)((float)quantised(w[(size_t)f * m + j], s_inv[c0 + i]) * s_scale[c0 + i]) : (__bf16)0.f;
+            for (int i = 0; i < 8; ++i) {
+                const int j = 64 * T + c0 + i;
+                o[i] = (j < m && f < k) ? (__bf16)((float)quantised(w[(size_t)f * m + j], s_inv[c0 + i]) * s_scale[c0 + i]) : (__bf16)0.f;
+            }
+            *(bf16x8*)(packed + lay.frags_t + ((((size_t)s * msteps + 2 * T + half) * 4 + u) * 64 + lane) * 16) = o;
         }
-        *(bf16x8*)(packed + lay.frags_t + ((((size_t)tf * msteps + 2 * T + (q & 1)) * 4 + u) * 64 + lane) * 16) = o;
     }
 }
 
@@ -146,9 +147,8 @@ NERF_API int nerf_int8_pack(const float* w, int k, int m, int pow2, void* packed
     NERF_REQUIRE(k >= 1 && m >= 1 && k <= kMaxWidth && m <= kMaxWidth, "nerf_int8_pack: widths must be in [1, %d], got %d x %d", kMaxWidth, k, m);
     NERF_REQUIRE(((uintptr_t)packed & 15) == 0 && ((uintptr_t)w & 3) == 0, "nerf_int8_pack: misaligned pointer");
     const PackedLayout lay(k, m, pow2 != 0);
-    // four steps of 64 inputs per turn: one turn each, up to 32 workgroups per channel group
-    const int turns = (lay.kp / 64 + 3) / 4;
-    const dim3 grid(lay.mp / 64, turns < 32 ? turns : 32);
+    const int steps = lay.kp / 64;
+    const dim3 grid(lay.mp / 64, steps < 32 ? steps : 32);  // a step of 64 inputs each where there are that few
     int8_pack_kernel<<<grid, kPackThreads, 0, as_stream(stream)>>>(w, k, m, pow2, (char*)packed, lay);
     return check_launch("nerf_int8_pack");
 }

@@ -429,12 +429,17 @@ def _on_gpu(what, *tensors):
     return dev
 
 
+_ENTRY = {}   # name -> entry point of the library
+
+
 def _call(name, dev, *args):
     """One entry point on `dev` and its current stream; device pointers as integers.  (A call for one ray is
     all host time: no context manager and no stream object where the device is the current one.)"""
-    fn = getattr(nv.lib(), name)
+    fn = _ENTRY.get(name)
+    if fn is None:
+        fn = _ENTRY[name] = getattr(nv.lib(), name)
     index = dev.index
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
@@ -507,10 +512,15 @@ class Int8Weights:
         return f"Int8Weights(k={self.k}, m={self.m}, pow2={self.pow2})"
 
 
+def _new(shape, dtype, dev):
+    # (the cheapest of torch's allocations from Python)
+    return torch.empty_strided(shape, (shape[1], 1) if len(shape) == 2 else (1,), dtype=dtype, device=dev)
+
+
 def _new_rows(n, k, dev, want_mask):
     kp = _padded_width(k)
-    return (torch.empty((n, kp), dtype=torch.int8, device=dev), torch.empty((n,), dtype=torch.float32, device=dev),
-            torch.empty((n, kp // 8), dtype=torch.uint8, device=dev) if want_mask else None)
+    return (_new((n, kp), torch.int8, dev), _new((n,), torch.float32, dev),
+            _new((n, kp // 8), torch.uint8, dev) if want_mask else None)
 
 
 def quantize_rows(x, pow2=False, want_mask=False):
@@ -532,13 +542,14 @@ def pack_int8(w, pow2=False, into=None):
     dev = _on_gpu("pack_int8", w)
     if w.dim() != 2 or w.shape[0] < 1 or w.shape[1] < 1:
         raise ValueError(f"pack_int8: expected [k >= 1, m >= 1], got {tuple(w.shape)}")
-    w = nv.f32(w.detach(), dev)
+    if w.dtype != torch.float32 or not w.is_contiguous():
+        w = nv.f32(w.detach(), dev)
     k, m = w.shape
-    need = int(nv.lib().nerf_int8_packed_bytes(k, m, int(bool(pow2))))
+    need = nv.lib().nerf_int8_packed_bytes(k, m, 1 if pow2 else 0)
     if need == 0:
         raise ValueError(f"pack_int8: widths {k} x {m} are beyond what the kernels are built for")
     if into is None:
-        packed = torch.empty((need,), dtype=torch.uint8, device=dev)
+        packed = _new((need,), torch.uint8, dev)
     elif not isinstance(into, Int8Weights) or (into.k, into.m, into.pow2, into.packed.device) != (k, m, bool(pow2), dev):
         raise ValueError(f"pack_int8: into={into!r} does not hold {k} x {m} weights, pow2={bool(pow2)}, on {dev}")
     else:
@@ -576,7 +587,7 @@ def linear_int8(rows, weights, bias=None, relu=False, addend=None, dtype=torch.f
     if dtype not in _DTYPES:
         raise ValueError(f"linear_int8: dtype must be float32, float16 or bfloat16, got {dtype}")
     n, m = rows.n, weights.m
-    y = torch.empty((n, m), dtype=dtype, device=dev)
+    y = _new((n, m), dtype, dev)
     _call("nerf_linear_int8", dev, rows.q.data_ptr(), rows.scale.data_ptr(), n, rows.k, weights.packed.data_ptr(), m, _addr(bias),
           _addr(addend), add_dtype, ldadd, 1 if relu else 0, y.data_ptr(), _DTYPES[dtype], m)
     return y
@@ -611,7 +622,7 @@ def linear_int8_grad_input(dz, weights, mask=None):
         mask = mask.contiguous()
     if mask is not None and (mask.dtype != torch.uint8 or tuple(mask.shape) != (n, _padded_width(weights.k) // 8)):
         raise ValueError(f"{what}: mask must be uint8 [{n}, {_padded_width(weights.k) // 8}], got {mask.dtype} {tuple(mask.shape)}")
-    dx = torch.empty((n, weights.k), dtype=dz.dtype, device=dev)
+    dx = _new((n, weights.k), dz.dtype, dev)
     _call("nerf_linear_int8_grad_input", dev, dz.data_ptr(), _DTYPES[dz.dtype], n, weights.m, ld, weights.packed.data_ptr(), weights.k,
           _addr(mask), dx.data_ptr(), weights.k)
     return dx
@@ -632,10 +643,9 @@ def linear_int8_grad_weight(rows, dz):
         raise ValueError(f"{what}: {rows.n} rows against {n} of dz")
     if n == 0:
         return (torch.zeros((rows.k, m), dtype=torch.float32, device=dev), torch.zeros((m,), dtype=torch.float32, device=dev))
-    dw = torch.empty((rows.k, m), dtype=torch.float32, device=dev)
-    db = torch.empty((m,), dtype=torch.float32, device=dev)
-    need = int(nv.lib().nerf_linear_int8_grad_weight_bytes(n, rows.k, m))
-    ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+    dw, db = _new((rows.k, m), torch.float32, dev), _new((m,), torch.float32, dev)
+    need = nv.lib().nerf_linear_int8_grad_weight_bytes(n, rows.k, m)
+    ws = _new((need,), torch.uint8, dev) if need else None
     _call("nerf_linear_int8_grad_weight", dev, rows.q.data_ptr(), rows.scale.data_ptr(), n, rows.k, dz.data_ptr(), _DTYPES[dz.dtype], m,
           ld, dw.data_ptr(), db.data_ptr(), _addr(ws), need)
     return dw, db
