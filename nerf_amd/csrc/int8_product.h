@@ -282,18 +282,6 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int T0 = blockIdx.y * NT;
 
-    // fragments [group][step] -> LDS [step][group]; groups behind the last are zeros
-    {
-        const i32x4* src = (const i32x4*)(a.frags + (size_t)T0 * a.frag_steps * 4096);
-        for (int i = threadIdx.x; i < NT * a.steps * 256; i += kResidentThreads) {
-            const int T = i / (a.steps * 256), s = (i >> 8) - T * a.steps;
-            *(i32x4*)(wl + ((s * NT + T) * 256 + (i & 255)) * 16) =
-                T0 + T < a.groups ? src[(T * a.frag_steps + s) * 256 + (i & 255)] : i32x4{0, 0, 0, 0};
-        }
-        if constexpr (Op::kInt8) stage_channels(a, ws, bs, 64 * T0, NT * 64);
-    }
-    __syncthreads();
-
     // what the work on a tile's sums reads of its rows: requested with them, not when it is needed (that
     // wait would also be one for the next unit's rows)
     struct Side {
@@ -425,10 +413,19 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
         }
     };
 
+    // The first rows are requested, then the fragments are copied, [group][step] -> LDS [step][group], without
+    // passing registers (a group behind the last repeats it and is not stored), all before the first wait.
     const int64_t stride = (int64_t)gridDim.x * (kResidentThreads / 64);
     int64_t tile = (int64_t)blockIdx.x * (kResidentThreads / 64) + wave;
     int s0 = 0;
-    if (tile < tiles) fetch(tile, 0, raw[0]);
+    fetch(tile < tiles ? tile : tiles - 1, 0, raw[0]);
+    for (int i = wave; i < NT * a.steps * 4; i += kResidentThreads / 64) {
+        const int s = i / (NT * 4), T = (i >> 2) % NT, t = T0 + T < a.groups ? T0 + T : a.groups - 1;
+        glds16_untracked(a.frags + ((size_t)t * a.frag_steps + s) * 4096 + (i & 3) * 1024 + lane * 16, wl + i * 1024);
+    }
+    if constexpr (Op::kInt8) stage_channels(a, ws, bs, 64 * T0, NT * 64);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
     while (tile < tiles) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
