@@ -143,65 +143,6 @@ DEV Raw8<T> load8(const T* row, int c, int width, bool whole) {
     return r;
 }
 
-// Elements f .. f + 15 of a row of `width`, as far as they exist; `whole` as above.  A piece that passes the
-// end leaves as runs of 8, 4, 2 and 1 elements.
-template <class T>
-DEV void store16(T* row, int f, int width, bool whole, const float (&v)[16]) {
-    constexpr int W = sizeof(T) == 4 ? 16 : 8;
-    int w[W];
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-        if constexpr (W == 16) {
-            w[i] = __builtin_bit_cast(int, v[i]);
-        } else {
-            typedef T pair __attribute__((ext_vector_type(2)));
-            const pair t = {(T)v[2 * i], (T)v[2 * i + 1]};
-            w[i] = __builtin_bit_cast(int, t);
-        }
-    }
-    char* dst = (char*)(row + f);
-    if (whole || f + 16 <= width) {
-#pragma unroll
-        for (int i = 0; i < W / 4; ++i) *(i32x4u*)(dst + 16 * i) = i32x4{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
-        return;
-    }
-    const int have = width - f;
-    if (have <= 0) return;
-    constexpr int kRun8 = W / 2;  // words of 8 elements
-    if (have & 8) {
-#pragma unroll
-        for (int i = 0; i < kRun8 / 4; ++i) *(i32x4u*)(dst + 16 * i) = i32x4{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
-        dst += 4 * kRun8;
-#pragma unroll
-        for (int i = 0; i < kRun8; ++i) w[i] = w[i + kRun8];
-    }
-    if constexpr (W == 16) {
-        if (have & 4) {
-            *(i32x4u*)dst = i32x4{w[0], w[1], w[2], w[3]};
-            dst += 16;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = w[i + 4];
-        }
-        if (have & 2) {
-            typedef int i32x2 __attribute__((ext_vector_type(2)));
-            *(i32x2u*)dst = i32x2{w[0], w[1]};
-            dst += 8, w[0] = w[2];
-        }
-        if (have & 1) *(i32u*)dst = w[0];
-    } else {
-        if (have & 4) {
-            typedef int i32x2 __attribute__((ext_vector_type(2)));
-            *(i32x2u*)dst = i32x2{w[0], w[1]};
-            dst += 8, w[0] = w[2], w[1] = w[3];
-        }
-        if (have & 2) {
-            *(i32u*)dst = w[0];
-            dst += 4, w[0] = w[1];
-        }
-        if (have & 1) *(unsigned short*)dst = (unsigned short)w[0];
-    }
-}
-
 // N consecutive elements at p (any alignment the element type allows) as floats; only the first `have`
 // exist, the others read as zero.
 template <class T, int N>

@@ -44,7 +44,7 @@ NERF_API int nerf_linear_int8_grad_input(const void* dz, int dtype, int64_t n, i
     NERF_REQUIRE(dz && packed && dx, "%s: null pointer", what);
     NERF_REQUIRE(lddz >= m && lddx >= k, "%s: rows overlap", what);
     NERF_REQUIRE(((uintptr_t)packed & 15) == 0 && (((uintptr_t)dz | (uintptr_t)dx) & (dtype_size(dtype) - 1)) == 0 &&
-                     ((uintptr_t)mask & 1) == 0,
+                     ((uintptr_t)mask & 7) == 0,
                  "%s: misaligned pointer", what);
     const PackedLayout lay(k, m, true);
     LinearArgs a{};

@@ -1,10 +1,12 @@
 // Products of rows with packed weights, shared by int8_linear.hip (8-bit integers, int32 sums) and
 // int8_grad_input.hip (bf16 terms, fp32 sums).  Formats: int8_common.h.
 //
-// Both are D[feature][point] = sum over the contraction of A[feature][c] B[c][point] with 16 x 16 tiles:
-// A fragments are stored as the matrix unit takes them, a lane's B fragment is 16 integers (8 bf16)
-// that lie next to each other in its point's row, and the four tiles of a group of 64 features leave
-// 16 neighbouring features of one point in a lane.
+// Both are D[feature][point] = sum over the contraction of A[feature][c] B[c][point] with 16 x 16 tiles: a
+// lane's B fragment is 16 integers (8 bf16) that lie next to each other in its point's row.  Which
+// features a tile has is a matter of the rows its A fragment is read with (frag_source): the four tiles of
+// a group of 64 features leave a lane (point = lane & 15, g = lane >> 4) pieces of 16 bytes of the
+// output, 4, 8 or 16 neighbouring features, and the four lanes of a point pieces that are neighbours, so
+// that every store covers 64-byte runs.
 #pragma once
 #include "int8_common.h"
 #include "mlp_common.h"
@@ -97,15 +99,84 @@ struct Bf16Op {
     }
 };
 
-// ---- what becomes of the sums of a lane: 16 neighbouring features of point p -------------------------
-template <class T>
-DEV void add16(const T* row, int f, int width, bool whole, float (&v)[16]) {
+// ---- which features a lane has -------------------------------------------------------------------------
+template <int OUT> constexpr int kPiece = OUT == NERF_F32 ? 4 : OUT < TO_INT8 ? 8 : 16;
+
+// Feature, inside its group of 64, of value i of a lane (accumulator i >> 2, register i & 3).
+template <int OUT>
+DEV int feature_of(int i, int g) {
+    return (i / kPiece<OUT>) * (4 * kPiece<OUT>) + g * kPiece<OUT> + i % kPiece<OUT>;
+}
+// Where, in the four stored fragments of a group and step, a lane finds its row of A for tile u.
+template <int OUT>
+DEV int frag_source(int u, int lane) {
+    const int f = feature_of<OUT>(4 * u + (lane & 3), (lane >> 2) & 3);
+    return ((f >> 2) & 3) * 1024 + (4 * (f >> 4) + (f & 3) + (lane & 48)) * 16;
+}
+
+// ---- what becomes of the sums of a lane ------------------------------------------------------------------
+// N neighbouring elements of a row added to v; `whole` (the same in every lane): all of them exist.
+template <class A, int N>
+DEV void add_piece(const A* p, int have, bool whole, float* v) {
+    if (whole) {
+        constexpr int W = N * sizeof(A) / 4;
+        int w[W];
+        if constexpr (W == 2) {
+            typedef int i32x2 __attribute__((ext_vector_type(2)));
+            const i32x2 q = *(const i32x2u*)p;
+            w[0] = q[0], w[1] = q[1];
+        } else {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        float d[8];
-        to_float(load8<T>(row, f + 8 * h, width, whole), d);
+            for (int i = 0; i < W / 4; ++i) {
+                const i32x4 q = *(const i32x4u*)((const char*)p + 16 * i);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[8 * h + i] += d[i];
+                for (int j = 0; j < 4; ++j) w[4 * i + j] = q[j];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if constexpr (sizeof(A) == 4) v[i] += __builtin_bit_cast(float, w[i]);
+            else v[i] += __builtin_bit_cast(float, (i & 1) ? w[i >> 1] & (int)0xffff0000 : w[i >> 1] << 16);  // bf16
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i < have) v[i] += (float)p[i];
+    }
+}
+
+// 16 bytes of a row, as far as its elements exist: a piece that passes the end leaves as runs of 4, 2 and 1.
+template <class T, int N>
+DEV void store_piece(T* dst, int have, bool whole, const float* v) {
+    int w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (N == 4) {
+            w[i] = __builtin_bit_cast(int, v[i]);
+        } else {
+            typedef T pair __attribute__((ext_vector_type(2)));
+            const pair t = {(T)v[2 * i], (T)v[2 * i + 1]};
+            w[i] = __builtin_bit_cast(int, t);
+        }
+    }
+    if (whole || have >= N) {
+        *(i32x4u*)dst = i32x4{w[0], w[1], w[2], w[3]};
+        return;
+    }
+    if (have <= 0) return;
+    typedef int i32x2 __attribute__((ext_vector_type(2)));
+    char* d = (char*)dst;
+    const int words = have * (int)sizeof(T) / 4;
+    if (words & 2) {
+        *(i32x2u*)d = i32x2{w[0], w[1]};
+        d += 8, w[0] = w[2], w[1] = w[3];
+    }
+    if (words & 1) {
+        *(i32u*)d = w[0];
+        d += 4, w[0] = w[1];
+    }
+    if constexpr (N == 8) {
+        if (have & 1) *(unsigned short*)d = (unsigned short)w[0];
     }
 }
 
@@ -114,19 +185,26 @@ DEV float positive_nan(float v) { return v != v ? __builtin_bit_cast(float, 0x7f
 
 // y = relu((sum x channel scale) x row scale + bias + addend): the sum rounded to fp32, its product with
 // the channel scale rounded, then one rounding for row scale and bias and one for the addend.  ws, b: the
-// 16 channels' scales and biases (0 and 0 behind the last channel; a NaN without its sign).
-template <int ADD>
-DEV void finish_linear(const LinearArgs& a, const i32x4 (&acc)[4], const float* ws, const float* b, float xs, int f, int64_t p,
-                       bool whole, bool relu, float (&v)[16]) {
+// channels' scales and biases of the group of 64 from f0 (0 and 0 behind the last channel; a NaN without
+// its sign).
+template <int OUT, int ADD>
+DEV void finish_linear(const LinearArgs& a, const i32x4 (&acc)[4], const float* ws, const float* b, float xs, int f0, int g,
+                       int64_t p, bool whole, bool relu, float (&v)[16]) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-        const f32x4 w4 = *(const f32x4*)(ws + 4 * u), b4 = *(const f32x4*)(b + 4 * u);
+        const int f = feature_of<OUT>(4 * u, g);
+        const f32x4 w4 = *(const f32x4*)(ws + f), b4 = *(const f32x4*)(b + f);
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[4 * u + r] = __builtin_fmaf((float)acc[u][r] * w4[r], xs, b4[r]);
     }
     if constexpr (ADD != NO_ADD) {
         typedef typename Elem<ADD>::T A;
-        add16((const A*)a.addend + p * a.ldadd, f, a.features, whole, v);
+        const A* row = (const A*)a.addend + p * a.ldadd;
+#pragma unroll
+        for (int i = 0; i < 16; i += kPiece<OUT>) {
+            const int f = f0 + feature_of<OUT>(i, g);
+            add_piece<A, kPiece<OUT>>(row + f, a.features - f, whole, v + i);
+        }
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = positive_nan(v[i]);
     }
@@ -171,25 +249,34 @@ DEV uint4 round16(const float (&v)[16], float inv) {
     return inv == 0.f ? make_uint4(0u, 0u, 0u, 0u) : make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-template <int DT>
-DEV void put(const LinearArgs& a, int64_t p, int f, bool whole, const float (&v)[16]) {
-    typedef typename Elem<DT>::T O;
-    store16<O>((O*)a.out + p * a.ldout, f, a.features, whole, v);
+template <int OUT>
+DEV void put(const LinearArgs& a, int64_t p, int f0, int g, bool whole, const float (&v)[16]) {
+    typedef typename Elem<OUT>::T O;
+    O* row = (O*)a.out + p * a.ldout;
+#pragma unroll
+    for (int i = 0; i < 16; i += kPiece<OUT>) {
+        const int f = f0 + feature_of<OUT>(i, g);
+        store_piece<O, kPiece<OUT>>(row + f, a.features - f, whole, v + i);
+    }
 }
 
-// Bits of the mask of features f .. f + 15 of point p (rows of bits are padded like rows of integers).
-DEV unsigned mask_bits(const LinearArgs& a, int64_t p, int f) {
-    return a.mask ? *(const unsigned short*)(a.mask + p * (a.groups * 8) + f / 8) : 0xffffu;
+// The 64 bits of a group of features, moved so that a lane's own are at places that do not depend on it.
+template <int OUT>
+DEV uint2 own_bits(uint2 m, int g) {
+    return make_uint2(m.x >> (g * kPiece<OUT>), m.y >> (g * kPiece<OUT>));
 }
 
-template <int DT>
-DEV void put_grad(const LinearArgs& a, const f32x4 (&acc)[4], int f, int64_t p, bool whole, unsigned bits) {
+template <int OUT>
+DEV void put_grad(const LinearArgs& a, const f32x4 (&acc)[4], int f0, int g, int64_t p, bool whole, uint2 own) {
     float v[16];
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[4 * u + r] = bits >> (4 * u + r) & 1 ? acc[u][r] : 0.f;
-    put<DT>(a, p, f, whole, v);
+    for (int i = 0; i < 16; ++i) {
+        const int at = (i / kPiece<OUT>) * (4 * kPiece<OUT>) + i % kPiece<OUT>;  // of 64, but for the lane's shift
+        const float x = acc[i >> 2][i & 3];
+        const int keep = __builtin_amdgcn_sbfe((int)(at < 32 ? own.x : own.y), at & 31, 1);  // all ones or none
+        v[i] = __builtin_bit_cast(float, __builtin_bit_cast(int, x) & keep);
+    }
+    put<OUT>(a, p, f0, g, whole, v);
 }
 
 // Channel scales and biases of `count` features from f0 into LDS, zeros behind the last.
@@ -204,7 +291,7 @@ DEV void stage_channels(const LinearArgs& a, float* ws, float* b, int f0, int co
 // ---- kernels --------------------------------------------------------------------------------------------
 
 // Few rows: one wave per group of 64 features x 32 points, operands straight from global memory.
-template <class Op, int DT, int ADD>
+template <class Op, int OUT, int ADD>
 __global__ __launch_bounds__(256) void linear_direct_kernel(LinearArgs a) {
     constexpr int P = 2;
     __shared__ __attribute__((aligned(16))) float ch[4][2][64];
@@ -224,14 +311,17 @@ __global__ __launch_bounds__(256) void linear_direct_kernel(LinearArgs a) {
         const int64_t p = p0 + 16 * j + r;
         row[j] = p < a.n ? p : a.n - 1;  // a lane behind the last row repeats it and stores nothing
     }
-    const char* w = a.frags + (size_t)T * a.frag_steps * 4096 + lane * 16;
+    const char* w = a.frags + (size_t)T * a.frag_steps * 4096;
+    int at[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) at[u] = frag_source<OUT>(u, lane);
     for (int s = 0; s < a.steps; ++s, w += 4096) {
         typename Op::Raw raw[P];
 #pragma unroll
         for (int j = 0; j < P; ++j) raw[j] = Op::fetch(a, row[j], s, g);
         i32x4 wf[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) wf[u] = *(const i32x4*)(w + u * 1024);
+        for (int u = 0; u < 4; ++u) wf[u] = *(const i32x4*)(w + at[u]);
 #pragma unroll
         for (int j = 0; j < P; ++j) {
             const typename Op::B b(raw[j]);
@@ -239,7 +329,6 @@ __global__ __launch_bounds__(256) void linear_direct_kernel(LinearArgs a) {
             for (int u = 0; u < 4; ++u) acc[j][u] = Op::mma(wf[u], b, acc[j][u]);
         }
     }
-    const int f = 64 * T + 16 * g;
     const bool whole = 64 * T + 64 <= a.features;
     if constexpr (Op::kInt8) {
         // this wave's 64 channels, through its own piece of LDS (one wave: in order, no barrier)
@@ -250,13 +339,15 @@ __global__ __launch_bounds__(256) void linear_direct_kernel(LinearArgs a) {
 #pragma unroll
         for (int j = 0; j < P; ++j) {
             float v[16];
-            finish_linear<ADD>(a, acc[j], &ch[wave][0][16 * g], &ch[wave][1][16 * g], a.scale[row[j]], f, row[j], whole, a.relu != 0, v);
-            if (p0 + 16 * j + r < a.n) put<DT>(a, row[j], f, whole, v);
+            finish_linear<OUT, ADD>(a, acc[j], ch[wave][0], ch[wave][1], a.scale[row[j]], 64 * T, g, row[j], whole, a.relu != 0, v);
+            if (p0 + 16 * j + r < a.n) put<OUT>(a, row[j], 64 * T, g, whole, v);
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < P; ++j)
-            if (p0 + 16 * j + r < a.n) put_grad<DT>(a, acc[j], f, row[j], whole, mask_bits(a, row[j], f));
+        for (int j = 0; j < P; ++j) {
+            const uint2 m = a.mask ? *(const uint2*)(a.mask + row[j] * (a.groups * 8) + 8 * T) : make_uint2(~0u, ~0u);
+            if (p0 + 16 * j + r < a.n) put_grad<OUT>(a, acc[j], 64 * T, g, row[j], whole, own_bits<OUT>(m, g));
+        }
     }
 }
 
@@ -286,7 +377,7 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
     // wait would also be one for the next unit's rows)
     struct Side {
         float xs;
-        unsigned bits[NT];
+        uint2 bits[NT];
     };
     typename Op::Raw raw[2][CH][P];
     Side side[2][P];  // of the tile being worked on, of the one being fetched
@@ -298,7 +389,7 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
     // bits of the mask: without one, any bytes, all set afterwards
     const unsigned char* const mask = a.mask ? a.mask : (const unsigned char*)a.frags;
     const int64_t mask_ld = a.mask ? a.groups * 8 : 0;
-    const unsigned no_mask = a.mask ? 0u : 0xffffu;
+    const unsigned no_mask = a.mask ? 0u : ~0u;
     auto fetch = [&](int64_t tile, int s0, typename Op::Raw (&to)[CH][P]) {
 #pragma unroll
         for (int j = 0; j < P; ++j) {
@@ -309,7 +400,8 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
 #pragma unroll
                 for (int T = 0; T < NT; ++T) {
                     const int t = T0 + T < a.groups ? T0 + T : a.groups - 1;
-                    side[1][j].bits[T] = *(const unsigned short*)(mask + p * mask_ld + 8 * t + 2 * g) | no_mask;
+                    const uint2 m = *(const uint2*)(mask + p * mask_ld + 8 * t);
+                    side[1][j].bits[T] = make_uint2(m.x | no_mask, m.y | no_mask);
                 }
             }
 #pragma unroll
@@ -352,18 +444,17 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
 #pragma unroll
                     for (int T = 0; T < NT; ++T) {
                         if (T0 + T < a.groups)
-                            put_grad<OUT>(a, acc[j][T], 64 * (T0 + T) + 16 * g, p, 64 * (T0 + T) + 64 <= a.features, now.bits[T]);
+                            put_grad<OUT>(a, acc[j][T], 64 * (T0 + T), g, p, 64 * (T0 + T) + 64 <= a.features, own_bits<OUT>(now.bits[T], g));
                     }
                 }
             } else if constexpr (OUT < TO_INT8) {
 #pragma unroll
                 for (int T = 0; T < NT; ++T) {
-                    const int f = 64 * (T0 + T) + 16 * g;
                     const bool whole = 64 * (T0 + T) + 64 <= a.features;
                     if (T0 + T < a.groups && live) {
                         float v[16];
-                        finish_linear<ADD>(a, acc[j][T], ws + 64 * T + 16 * g, bs + 64 * T + 16 * g, now.xs, f, p, whole, a.relu != 0, v);
-                        put<OUT>(a, p, f, whole, v);
+                        finish_linear<OUT, ADD>(a, acc[j][T], ws + 64 * T, bs + 64 * T, now.xs, 64 * (T0 + T), g, p, whole, a.relu != 0, v);
+                        put<OUT>(a, p, 64 * (T0 + T), g, whole, v);
                     }
                     __builtin_amdgcn_sched_barrier(0);  // in turn: 16 sums become 16 values in the same registers
                 }
@@ -375,8 +466,7 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
 #pragma unroll
                 for (int T = 0; T < NT; ++T) {
                     if (T < a.groups) {  // (an addend's rows are whole groups here)
-                        finish_linear<ADD>(a, acc[j][T], ws + 64 * T + 16 * g, bs + 64 * T + 16 * g, now.xs, 64 * T + 16 * g, p, true,
-                                           RELU, v[T]);
+                        finish_linear<OUT, ADD>(a, acc[j][T], ws + 64 * T, bs + 64 * T, now.xs, 64 * T, g, p, true, RELU, v[T]);
                     } else {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) v[T][i] = 0.f;
@@ -419,9 +509,10 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
     int64_t tile = (int64_t)blockIdx.x * (kResidentThreads / 64) + wave;
     int s0 = 0;
     fetch(tile < tiles ? tile : tiles - 1, 0, raw[0]);
+    const int lane_source = frag_source<OUT>(wave & 3, lane);  // this wave copies tile wave & 3 of every group and step
     for (int i = wave; i < NT * a.steps * 4; i += kResidentThreads / 64) {
         const int s = i / (NT * 4), T = (i >> 2) % NT, t = T0 + T < a.groups ? T0 + T : a.groups - 1;
-        glds16_untracked(a.frags + ((size_t)t * a.frag_steps + s) * 4096 + (i & 3) * 1024 + lane * 16, wl + i * 1024);
+        glds16_untracked(a.frags + ((size_t)t * a.frag_steps + s) * 4096 + lane_source, wl + i * 1024);
     }
     if constexpr (Op::kInt8) stage_channels(a, ws, bs, 64 * T0, NT * 64);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -480,7 +571,7 @@ __global__ __launch_bounds__(kStreamThreads) void linear_streamed_kernel(LinearA
     for (int i = 0; i < 4; ++i) {
         if (wave < 4) {
             const int T = T0 + wave < a.groups ? T0 + wave : a.groups - 1;  // a group behind the last is not stored
-            src[i] = a.frags + (size_t)T * a.frag_steps * 4096 + i * 1024 + lane * 16;
+            src[i] = a.frags + (size_t)T * a.frag_steps * 4096 + frag_source<OUT>(i, lane);
         } else {
             int64_t p = pb * 256 + ((wave - 4) * 4 + i) * 16 + r;
             if (p >= a.n) p = a.n - 1;
@@ -541,15 +632,16 @@ __global__ __launch_bounds__(kStreamThreads) void linear_streamed_kernel(LinearA
         if constexpr (Op::kInt8) xs = a.scale[pc];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const int T = 2 * wf + t, f = 64 * (T0 + T) + 16 * g;
+            const int T = 2 * wf + t;
             const bool whole = 64 * (T0 + T) + 64 <= a.features;
             if (T0 + T < a.groups) {
                 if constexpr (Op::kInt8) {
                     float v[16];
-                    finish_linear<ADD>(a, acc[j][t], ws + 64 * T + 16 * g, bs + 64 * T + 16 * g, xs, f, pc, whole, a.relu != 0, v);
-                    if (live) put<OUT>(a, pc, f, whole, v);
+                    finish_linear<OUT, ADD>(a, acc[j][t], ws + 64 * T, bs + 64 * T, xs, 64 * (T0 + T), g, pc, whole, a.relu != 0, v);
+                    if (live) put<OUT>(a, pc, 64 * (T0 + T), g, whole, v);
                 } else if (live) {
-                    put_grad<OUT>(a, acc[j][t], f, pc, whole, mask_bits(a, pc, f));
+                    const uint2 m = a.mask ? *(const uint2*)(a.mask + pc * (a.groups * 8) + 8 * (T0 + T)) : make_uint2(~0u, ~0u);
+                    put_grad<OUT>(a, acc[j][t], 64 * (T0 + T), g, pc, whole, own_bits<OUT>(m, g));
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
