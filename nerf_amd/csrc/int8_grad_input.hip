@@ -25,6 +25,7 @@ static int launch(const LinearArgs& a, const char* what, hipStream_t st) {
     }
     if (a.n < kResidentRows || nt == 0) return launch_direct<Bf16Op<DT, false>, DT, NO_ADD>(a, what, st);
     if (nt == 4) return resident<DT, 4>(a, what, st);
+    if (nt == 3) return resident<DT, 3>(a, what, st);
     if (nt == 2) return resident<DT, 2>(a, what, st);
     return resident<DT, 1>(a, what, st);
 }

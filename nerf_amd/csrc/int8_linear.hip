@@ -32,7 +32,7 @@ static int launch(const LinearArgs& a, const char* what, hipStream_t st) {
         if (a.n < kResidentRows) return launch_direct<Int8Op, OUT, ADD>(a, what, st);
         if (nt == 0 || a.groups > nt) return launch_streamed<Int8Op, OUT, ADD>(a, what, st);
     }
-    if (nt == 4) return resident<OUT, 4, ADD>(a, what, st);
+    if (nt >= 3) return resident<OUT, 4, ADD>(a, what, st);  // (three groups only where they are all: one is idle)
     if (nt == 2) return resident<OUT, 2, ADD>(a, what, st);
     return resident<OUT, 1, ADD>(a, what, st);
 }

@@ -160,6 +160,19 @@ DEV void store_piece(T* dst, int have, bool whole, const float* v) {
         }
     }
     if (whole || have >= N) {
+        if constexpr (N == 8) {
+            // a row that starts between two words: the words inside the piece as such, half of one at each end
+            // (a vector store is slow there only)
+            if ((uintptr_t)dst & 2) {
+                typedef int i32x3u __attribute__((ext_vector_type(3), aligned(4)));
+                char* d = (char*)dst;
+                *(unsigned short*)d = (unsigned short)w[0];
+                *(i32x3u*)(d + 2) = i32x3u{(int)__builtin_amdgcn_alignbit(w[1], w[0], 16), (int)__builtin_amdgcn_alignbit(w[2], w[1], 16),
+                                           (int)__builtin_amdgcn_alignbit(w[3], w[2], 16)};
+                *(unsigned short*)(d + 14) = (unsigned short)((unsigned)w[3] >> 16);
+                return;
+            }
+        }
         *(i32x4u*)dst = i32x4{w[0], w[1], w[2], w[3]};
         return;
     }
@@ -696,15 +709,14 @@ inline int require_widths(const char* what, int64_t n, int k, int m) {
 }
 
 // Groups of features a workgroup of the resident kernel holds: as few feature blocks as LDS allows (each
-// reads the rows again), the groups spread evenly over them; 0: not even one group fits.
+// reads the rows again), the groups spread evenly over them (5 groups as 3 + 2 and not 4 + 1: every block
+// gets the same share of the CUs); 0: not even one group fits.
 inline int resident_groups(const LinearArgs& a) {
     int most = (kLdsBytes - channel_bytes<4>()) / (a.steps * 4096);
     if (most > 4) most = 4;
     if (most < 1) return 0;
     const int blocks = (a.groups + most - 1) / most;
-    int nt = (a.groups + blocks - 1) / blocks;
-    if (nt == 3 && most < 4) nt = 2;
-    return nt == 3 ? 4 : nt;
+    return (a.groups + blocks - 1) / blocks;
 }
 
 }  // namespace i8

@@ -453,3 +453,68 @@ def test_offsets_beyond_32_bits(gpu):
     dw, db = ops.linear_int8_grad_weight(rows, big)
     close(dw, xd.t().contiguous() @ d, xd.abs().t().contiguous() @ d.abs() * tail * 2.0 ** -23 + 1e-35, "dW")
     close(db, d.sum(0), d.abs().sum(0) * tail * 2.0 ** -23 + 1e-38, "db")
+
+
+@gpu_only
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n,k,m", [(40, 70, 96), (5000, 100, 96), (4500, 130, 33), (4200, 64, 3), (4200, 300, 222), (4096, 256, 256), (4300, 640, 600)])
+def test_a_row_that_is_not_finite_stays_one_row(gpu, n, k, m, dtype):
+    """A NaN in one row (in the middle, in the last) reaches that row's results and no other's, whatever the
+    width the rows are padded to."""
+    from nerf_amd import ops
+    x, w, dz, b = make(n, k, m, 9, gpu, TYPES[dtype])
+    packed = ops.pack_int8(w, True)
+    good = ops.linear_int8_grad_input(dz, packed)
+    goody = ops.linear_int8(ops.quantize_rows(x), packed, b)
+    for at in (n // 3, n - 1):
+        bad, badx = dz.clone(), x.clone()
+        bad[at, m // 2], badx[at, k // 2] = float("nan"), float("inf")
+        dx, y = ops.linear_int8_grad_input(bad, packed), ops.linear_int8(ops.quantize_rows(badx), packed, b)
+        rest = torch.arange(n, device=gpu) != at
+        assert bool(torch.isnan(dx[at]).all()) and torch.equal(dx[rest], good[rest])
+        assert bool(torch.isnan(y[at]).all()) and torch.equal(y[rest], goody[rest])
+
+
+@gpu_only
+@pytest.mark.parametrize("dt,t", [(0, torch.float32), (1, torch.float16), (2, torch.bfloat16)])
+@pytest.mark.parametrize("n,k,m", [(1, 5, 3), (37, 70, 19), (4100, 283, 130), (4099, 256, 256), (4100, 65, 600)])
+def test_nothing_else_is_written(gpu, n, k, m, dt, t):
+    """The C entry points on buffers with room between and behind the rows: what is not theirs keeps its bytes."""
+    from nerf_amd import _native, ops
+    lib, st = _native.lib(), torch.cuda.current_stream().cuda_stream
+    x, w, dz, b = make(n, k, m, 6, gpu, t)
+    rows, packed = ops.quantize_rows(x, True, True), ops.pack_int8(w, True)
+    kp, mp = rows.q.shape[1], -(-m // 64) * 64
+
+    def fresh(r, c, dtype):
+        return torch.full((r, c), 77, dtype=dtype, device=gpu)
+    q, s, bits = fresh(n + 2, kp, torch.int8), fresh(n + 2, 1, torch.float32), fresh(n + 2, kp // 8, torch.uint8)
+    assert lib.nerf_quantize_rows(x.data_ptr(), dt, n, k, k, 1, q.data_ptr(), s.data_ptr(), bits.data_ptr(), st) == 0
+    assert torch.equal(q[:n], rows.q) and torch.equal(s[:n, 0], rows.scale) and torch.equal(bits[:n], rows.mask)
+    assert bool((q[n:] == 77).all()) and bool((s[n:] == 77).all()) and bool((bits[n:] == 77).all())
+    y = fresh(n + 2, m + 5, t)
+    assert lib.nerf_linear_int8(rows.q.data_ptr(), rows.scale.data_ptr(), n, k, packed.packed.data_ptr(), m, b.data_ptr(), None, 0, 0, 1,
+                                y.data_ptr(), dt, m + 5, st) == 0
+    assert torch.equal(y[:n, :m], ops.linear_int8(rows, packed, b, relu=True, dtype=t))
+    assert bool((y[n:] == 77).all()) and bool((y[:, m:] == 77).all())
+    if m <= 256:
+        yq, ys, yb = fresh(n + 2, mp, torch.int8), fresh(n + 2, 1, torch.float32), fresh(n + 2, mp // 8, torch.uint8)
+        assert lib.nerf_linear_int8_quantized(rows.q.data_ptr(), rows.scale.data_ptr(), n, k, packed.packed.data_ptr(), m, b.data_ptr(), None, 0,
+                                              0, 1, 1, yq.data_ptr(), ys.data_ptr(), yb.data_ptr(), st) == 0
+        ref = ops.linear_int8_quantized(rows, packed, b, relu=True, pow2=True, want_mask=True)
+        assert torch.equal(yq[:n], ref.q) and torch.equal(ys[:n, 0], ref.scale) and torch.equal(yb[:n], ref.mask)
+        assert bool((yq[n:] == 77).all()) and bool((ys[n:] == 77).all()) and bool((yb[n:] == 77).all())
+    dx = fresh(n + 2, k + 3, t)
+    assert lib.nerf_linear_int8_grad_input(dz.data_ptr(), dt, n, m, m, packed.packed.data_ptr(), k, rows.mask.data_ptr(), dx.data_ptr(), k + 3, st) == 0
+    assert torch.equal(dx[:n, :k], ops.linear_int8_grad_input(dz, packed, rows.mask))
+    assert bool((dx[n:] == 77).all()) and bool((dx[:, k:] == 77).all())
+    need = lib.nerf_linear_int8_grad_weight_bytes(n, k, m)
+    dw, db, ws = fresh(k + 1, m, torch.float32), fresh(m + 3, 1, torch.float32), fresh(need + 64, 1, torch.uint8)
+    assert lib.nerf_linear_int8_grad_weight(rows.q.data_ptr(), rows.scale.data_ptr(), n, k, dz.data_ptr(), dt, m, m, dw.data_ptr(), db.data_ptr(),
+                                            ws.data_ptr(), need, st) == 0
+    ref = ops.linear_int8_grad_weight(rows, dz)
+    assert torch.equal(dw[:k], ref[0]) and torch.equal(db[:m, 0], ref[1])
+    assert bool((dw[k:] == 77).all()) and bool((db[m:] == 77).all()) and bool((ws[need:] == 77).all())
+    packed2 = fresh(packed.packed.numel() + 64, 1, torch.uint8)
+    assert lib.nerf_int8_pack(w.data_ptr(), k, m, 1, packed2.data_ptr(), st) == 0
+    assert torch.equal(packed2[:-64, 0], packed.packed) and bool((packed2[-64:] == 77).all())
