@@ -348,6 +348,7 @@ __global__ __launch_bounds__(256) void linear_direct_kernel(LinearArgs a) {
         const int c = 64 * T + lane;
         ch[wave][0][lane] = c < a.features ? a.wscale[c] : 0.f;
         ch[wave][1][lane] = (a.bias && c < a.features) ? positive_nan(a.bias[c]) : 0.f;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int j = 0; j < P; ++j) {
@@ -369,9 +370,13 @@ __global__ __launch_bounds__(256) void linear_direct_kernel(LinearArgs a) {
 // the sums of all NT groups of a tile (16 NT P registers), so a row is read once, and its work is a run of
 // units: CH steps of a tile's rows.  While one unit is worked on, the next one's rows (of this tile or the
 // next) are on their way into the other half of the registers, so that loads are in flight all the
-// time; with bf16 rows, tiles of 32 points, which halve the reads of LDS, leave no room for that (786432 x 256 x 256,
-// input gradient: 249 us; 8-bit rows are small enough for two tiles of 16 and both halves).  A fetch is the same loads on every path (a step behind the last repeats it,
-// a tile behind the last repeats the one at hand): a wait for older loads counts the younger ones.
+// time; with bf16 rows, tiles of 32 points, which halve the reads of LDS, leave no room for that (786432 x
+// 256 x 256, input gradient: 249 us against 172; 8-bit rows are small enough for two tiles of 16 and both
+// halves).  A fetch is the same loads on every path (a step behind the last repeats it, a tile behind the
+// last repeats the one at hand): a wait for older loads counts the younger ones.
+// Bound by memory up to a few hundred inputs and outputs: 786432 x 256 x 256 bf16 input gradient 172 us
+// (4.8 TB/s), 262144 x 319 x 256 -> bf16 46 us (4.7 TB/s); with 8-bit output by vector instructions
+// (786432 x 256 x 256: 116 us, 3.6 TB/s, about 8 of them a value).
 constexpr int kResidentThreads = 512;
 template <int NT>
 constexpr int channel_bytes() { return 2 * NT * 64 * 4; }
@@ -561,7 +566,8 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
 // registers, three stages ahead; per stage a wave reads 12 fragments for 32 products, so the matrix
 // unit and not LDS sets the pace.  Rows must be 16-byte aligned and end with a step.  Workgroups 8 apart
 // run on the same die: they take the feature blocks of one block of rows in turn, which the die's L2
-// then holds.
+// then holds.  Bound by the matrix unit: 32768 x 2048 x 2048 144 us, 1.9 P op/s (weights and rows straight
+// from memory: 253 us).
 constexpr int kStreamThreads = 512, kStreamStages = 4, kStreamStage = 32 * 1024;
 
 template <class Op, int OUT, int ADD>

@@ -86,6 +86,7 @@ class _Pass:
         """pts [P, 3], viewdirs [P / S, 3], all fp32."""
         self.model = model
         packed = model.packed8()
+        self.version = model._packed8_version
         D = model.D
         pe = ops.quantize_rows(_encode(pts, model.input_ch), pow2=True)
         # one encoding per ray, its integers repeated for the ray's points
@@ -118,6 +119,8 @@ class _Pass:
     def gradients(self, d_raw):
         """Gradients of the parameters, in their order, from d raw [P, 4] fp32."""
         model, packed, D = self.model, self.model.packed8(), self.model.D
+        if model._packed8_version != self.version:
+            raise RuntimeError("the network's parameters changed between its forward and its backward pass")
         grads = [None] * len(model.params)
 
         def parameters(i, dz):
@@ -152,10 +155,12 @@ class _Pass:
 def query(model, pts, viewdirs, S):
     """raw [P, 4] of points [P, 3] with one view direction per S points, nothing recorded."""
     P = pts.shape[0]
+    if P == 0:
+        return pts.new_empty((0, 4))
     step = max(_QUERY_POINTS // S, 1)
     with torch.no_grad():
         out = [_Pass(model, pts[i * S:(i + step) * S], viewdirs[i:i + step], S).raw for i in range(0, P // S, step)]
-    return out[0] if len(out) == 1 else torch.cat(out, 0) if out else pts.new_empty((0, 4))
+    return out[0] if len(out) == 1 else torch.cat(out, 0)
 
 
 class LayeredQuery(torch.autograd.Function):
@@ -173,6 +178,8 @@ class LayeredQuery(torch.autograd.Function):
     @staticmethod
     def backward(ctx, d_raw):
         run, ctx.run = ctx.run, None
-        if d_raw is None or run is None:
+        if d_raw is None:  # the network's output did not reach the loss
             return (None, None, None) + (None,) * len(ctx.needs_input_grad[3:])
+        if run is None:
+            raise RuntimeError("backward through a network query a second time: its rows were released by the first")
         return (None, None, None) + tuple(run.gradients(nv.f32(d_raw).reshape(-1, 4)))

@@ -46,7 +46,7 @@ def run_network(inputs, viewdirs, fn, embed_fn, embeddirs_fn, netchunk=1024 * 64
     lead = tuple(pts.shape[:-1])
     if pts.dim() == 2:
         pts = pts[:, None, :]
-    pts = pts.reshape(pts.shape[0], -1, 3)
+    pts = pts.flatten(1, -2)
     vd = nv.f32(viewdirs, pts.device).reshape(-1, 3)
     if fn.layered:
         if vd.shape[0] != pts.shape[0]:

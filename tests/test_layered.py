@@ -227,3 +227,80 @@ def test_two_queries_of_one_network_and_unused_ones(gpu):
             LayeredQuery.apply(rays, x, net, *net.params)
             parts.append(tape.gradient((q * y).sum(), net.params))
     assert all(torch.equal(t, p + q) for t, p, q in zip(both, *parts))
+
+
+@gpu_only
+def test_backward_passes_that_cannot_be_right_raise(gpu):
+    from nerf_amd import training
+    from nerf_amd.layered import LayeredQuery
+    net = _net(gpu)
+    rays = torch.rand((9, 11), device=gpu)
+    z = torch.rand((9, 4), device=gpu).sort(1).values
+    with training.GradientTape():
+        raw = LayeredQuery.apply(rays, z, net, *net.params)
+        torch.autograd.grad(raw.sum(), net.params, retain_graph=True)
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(raw.sum(), net.params)
+        raw = LayeredQuery.apply(rays, z, net, *net.params)
+        net.set_weights([w * 2 for w in net.get_weights()])
+        with pytest.raises(RuntimeError, match="changed"):
+            torch.autograd.grad(raw.sum(), net.params)
+        raw = LayeredQuery.apply(rays, z, net, *net.params)       # ... and the network is as good as before
+        assert all(bool(torch.isfinite(g).all()) for g in torch.autograd.grad(raw.sum(), net.params))
+
+
+@gpu_only
+@pytest.mark.parametrize("n,S", [(0, 5), (3, 0), (0, 0)])
+def test_no_points(gpu, n, S):
+    from nerf_amd.run_nerf import create_nerf
+    kw = create_nerf(_args())[1]
+    raw = kw['network_query_fn'](torch.zeros((n, S, 3), device=gpu), torch.zeros((n, 3), device=gpu), kw['network_fn'])
+    assert raw.shape == (n, S, 4)
+
+
+def _alone_over_rccl(rank, port, tmp):
+    import os
+    import torch.distributed as dist
+    from nerf_amd import parallel, training
+    from nerf_amd.run_nerf import create_nerf, render
+    torch.cuda.set_device(0)
+    gpu = torch.device("cuda", 0)
+    try:
+        dist.init_process_group("nccl", init_method=f"tcp://127.0.0.1:{port}", rank=0, world_size=1, device_id=gpu)
+        dist.all_reduce(torch.ones(4, device=gpu))
+        torch.cuda.synchronize()
+    except Exception as e:  # no RCCL on this machine: nothing to test
+        open(os.path.join(tmp, "unavailable"), "w").write(repr(e))
+        return
+    try:
+        def run(exchange):
+            parallel.EXCHANGE_WHEN_ALONE = exchange
+            torch.manual_seed(9)
+            kw_train, _, _, grad_vars, models = create_nerf(_args())
+            nets = [models['model'], models['model_fine']]
+            opt = training.Adam(5e-4).bind_models(nets)
+            g = torch.Generator(device=gpu).manual_seed(5)
+            o = torch.nn.functional.normalize(torch.randn((64, 3), generator=g, device=gpu), dim=1) * 4
+            t = torch.rand((64, 3), generator=g, device=gpu)
+            fn = lambda r: render(8, 8, 9.0, chunk=1024, rays=r, near=2., far=6., retraw=True, **{**kw_train, 'perturb': 0.})
+            losses = [training.train_step(fn, (o, -o / 4), t, grad_vars, opt)[0] for _ in range(3)]
+            return torch.stack(losses), [n.flat.detach().clone() for n in nets]
+        plain, over = run(False), run(True)
+        assert torch.equal(plain[0], over[0]) and all(torch.equal(a, b) for a, b in zip(plain[1], over[1]))
+        open(os.path.join(tmp, "ok"), "w").write("ok")
+    finally:
+        parallel.EXCHANGE_WHEN_ALONE = False
+        dist.destroy_process_group()
+
+
+@gpu_only
+def test_data_parallel_step_over_rccl_with_one_rank(gpu, tmp_path):
+    """The exchanges of one rank are identities (64 rays: the ray-count weight is a power of two)."""
+    import socket
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    torch.multiprocessing.spawn(_alone_over_rccl, args=(port, str(tmp_path)), nprocs=1, join=True)
+    if (tmp_path / "unavailable").exists():
+        pytest.skip((tmp_path / "unavailable").read_text())
+    assert (tmp_path / "ok").exists()
