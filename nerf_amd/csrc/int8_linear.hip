@@ -27,12 +27,13 @@ static int resident(const LinearArgs& a, const char* what, hipStream_t st) {
 
 template <int OUT, int ADD>
 static int launch(const LinearArgs& a, const char* what, hipStream_t st) {
-    const int nt = resident_groups(a);
+    const int nt = a.groups == 3 ? 4 : a.groups;  // (of three groups' kernel one would be idle)
+    const bool fits = nt <= 4 && channel_bytes<4>() + (int64_t)nt * a.steps * 4096 <= kLdsBytes;
     if constexpr (OUT < TO_INT8) {
         if (a.n < kResidentRows) return launch_direct<Int8Op, OUT, ADD>(a, what, st);
-        if (nt == 0 || a.groups > nt) return launch_streamed<Int8Op, OUT, ADD>(a, what, st);
+        if (!fits) return launch_streamed<Int8Op, OUT, ADD>(a, what, st);
     }
-    if (nt >= 3) return resident<OUT, 4, ADD>(a, what, st);  // (three groups only where they are all: one is idle)
+    if (nt == 4) return resident<OUT, 4, ADD>(a, what, st);
     if (nt == 2) return resident<OUT, 2, ADD>(a, what, st);
     return resident<OUT, 1, ADD>(a, what, st);
 }
