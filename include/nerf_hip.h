@@ -322,8 +322,7 @@ int nerf_linear_int8(const signed char* q, const float* scale, int64_t n, int k,
                      void* y, int dtype, int64_t ldy, nerf_stream_t stream);
 
 /* nerf_quantize_rows of that y (in fp32, never stored): the next layer's rows, yq [n][m rounded up to 64].  For
- * m up to nerf_linear_int8_quantized_width(k) (256 for k up to 576, else 0), and with an addend m a
- * multiple of 64; otherwise NERF_E_UNSUPPORTED. */
+ * m up to nerf_linear_int8_quantized_width(k) (512), and with an addend m a multiple of 64; otherwise NERF_E_UNSUPPORTED. */
 int nerf_linear_int8_quantized_width(int k);
 int nerf_linear_int8_quantized(const signed char* q, const float* scale, int64_t n, int k, const void* packed, int m,
                                const float* bias, const void* addend, int addend_dtype, int64_t ldadd, int relu,

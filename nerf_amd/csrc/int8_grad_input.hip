@@ -21,7 +21,7 @@ static int launch(const LinearArgs& a, const char* what, hipStream_t st) {
     const int nt = resident_groups(a);
     if constexpr (DT == NERF_BF16) {
         if (a.n >= kResidentRows && (nt == 0 || a.groups > nt) && a.width % 32 == 0 && a.lddz % 8 == 0 && ((uintptr_t)a.dz & 15) == 0)
-            return launch_streamed<Bf16Op<DT, true>, DT, NO_ADD>(a, what, st);
+            return launch_streamed<Bf16Op<DT, true>, DT, NO_ADD, 2>(a, what, st);
     }
     if (a.n < kResidentRows || nt == 0) return launch_direct<Bf16Op<DT, false>, DT, NO_ADD>(a, what, st);
     if (nt == 4) return resident<DT, 4>(a, what, st);

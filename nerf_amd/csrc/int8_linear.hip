@@ -31,7 +31,11 @@ static int launch(const LinearArgs& a, const char* what, hipStream_t st) {
     const bool fits = nt <= 4 && channel_bytes<4>() + (int64_t)nt * a.steps * 4096 <= kLdsBytes;
     if constexpr (OUT < TO_INT8) {
         if (a.n < kResidentRows) return launch_direct<Int8Op, OUT, ADD>(a, what, st);
-        if (!fits) return launch_streamed<Int8Op, OUT, ADD>(a, what, st);
+        if (!fits) return launch_streamed<Int8Op, OUT, ADD, 2>(a, what, st);
+    } else if (!fits) {
+        // a whole row in one workgroup (262144 x 512 x 512: 150 us, through an fp32 row and quantize_rows 319)
+        if (a.groups > 4) return launch_streamed<Int8Op, OUT, ADD, 4>(a, what, st);
+        return launch_streamed<Int8Op, OUT, ADD, 2>(a, what, st);
     }
     if (nt == 4) return resident<OUT, 4, ADD>(a, what, st);
     if (nt == 2) return resident<OUT, 2, ADD>(a, what, st);
@@ -85,8 +89,7 @@ NERF_API int nerf_linear_int8(const signed char* q, const float* scale, int64_t 
 }
 
 NERF_API int nerf_linear_int8_quantized_width(int k) {
-    // all 256 channels of a row in one workgroup: four groups of fragments for every 64 inputs
-    return k >= 1 && up64(k) / 64 * 4 * 4096 + channel_bytes<4>() <= kLdsBytes ? 256 : 0;
+    return k >= 1 && k <= kMaxWidth ? 512 : 0;  // all channels of a row in one workgroup
 }
 
 NERF_API int nerf_linear_int8_quantized(const signed char* q, const float* scale, int64_t n, int k, const void* packed, int m,
@@ -96,7 +99,7 @@ NERF_API int nerf_linear_int8_quantized(const signed char* q, const float* scale
     LinearArgs a{};
     if (int rc = linear_args(a, what, q, scale, n, k, packed, m, bias, addend, addend_dtype, ldadd, relu)) return rc;
     if (m > nerf_linear_int8_quantized_width(k))
-        return NERF_FAIL(NERF_E_UNSUPPORTED, "%s: %d inputs and %d outputs do not fit one workgroup", what, k, m);
+        return NERF_FAIL(NERF_E_UNSUPPORTED, "%s: %d outputs do not fit one workgroup", what, m);
     if (addend && m % 64 != 0)
         return NERF_FAIL(NERF_E_UNSUPPORTED, "%s: an addend of %d columns is not a whole number of 64", what, m);
     if (n == 0) return 0;

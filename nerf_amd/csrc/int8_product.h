@@ -560,55 +560,71 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
     }
 }
 
-// Weights that do not fit LDS: a workgroup forms a tile of 256 features x 256 points, a wave 128 x 64 of
-// it (128 registers of sums).  The contraction goes through a ring of four stages of one step (16
-// fragments of weights, 16 of rows: 32 KiB), copied from global memory to LDS without passing
-// registers, three stages ahead; per stage a wave reads 12 fragments for 32 products, so the matrix
-// unit and not LDS sets the pace.  Rows must be 16-byte aligned and end with a step.  Workgroups 8 apart
-// run on the same die: they take the feature blocks of one block of rows in turn, which the die's L2
-// then holds.  Bound by the matrix unit: 32768 x 2048 x 2048 144 us, 1.9 P op/s (weights and rows straight
-// from memory: 253 us).
-constexpr int kStreamThreads = 512, kStreamStages = 4, kStreamStage = 32 * 1024;
+// Weights that do not fit LDS: a workgroup forms a tile of 128 FW features x 512 / FW points, a wave 128 x 64
+// of it (128 registers of sums), FW waves side by side along the features.  The contraction goes through a
+// ring of stages of one step (8 FW fragments of weights, 32 / FW of rows), copied from global memory to LDS
+// without passing registers, all but one stage ahead; per stage a wave reads 12 fragments for 32
+// products, so the matrix unit and not LDS sets the pace.  Rows must be 16-byte aligned and end with a
+// step.  Workgroups 8 apart run on the same die: they take the feature blocks of one block of rows in turn,
+// which the die's L2 then holds.  Bound by the matrix unit: 32768 x 2048 x 2048 144 us, 1.9 P op/s (weights
+// and rows straight from memory: 253 us).
+// FW 2: tiles of 256 x 256 and four stages of 32 KiB.  FW 4: 512 x 128 and three of 40 KiB, for 8-bit output of
+// more than 256 features, whose scale takes the whole row: the waves' maxima meet in LDS.
+constexpr int kStreamThreads = 512;
+template <int FW> constexpr int kStreamStages = FW == 2 ? 4 : 3;
+template <int FW> constexpr int kStreamStage = (8 * FW + 32 / FW) * 1024;
+template <int FW> constexpr int kStreamPoints = 512 / FW;
+template <int FW> constexpr int kStreamLds = 2 * 128 * FW * 4 + FW * kStreamPoints<FW> * 4 + kStreamStages<FW> * kStreamStage<FW>;
 
-template <class Op, int OUT, int ADD>
+template <class Op, int OUT, int ADD, int FW>
 __global__ __launch_bounds__(kStreamThreads) void linear_streamed_kernel(LinearArgs a, int fblocks, int64_t pblocks) {
+    static_assert(FW == 2 || FW == 4, "shapes");
+    constexpr int kFeatures = 128 * FW, kPoints = kStreamPoints<FW>, S = kStreamStages<FW>;
+    constexpr int C = (8 * FW + 32 / FW) / 8;  // copies of a wave for a stage
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float* const ws = (float*)lds;
-    float* const bs = ws + 256;
-    char* const ring = lds + 2 * 256 * 4;
+    float* const bs = ws + kFeatures;
+    unsigned* const tops = (unsigned*)(bs + kFeatures);  // [FW][kPoints]
+    char* const ring = (char*)(tops + FW * kPoints);
     const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int fb = (int)(blockIdx.x / 8 % fblocks);
     const int64_t pb = (int64_t)(blockIdx.x / 8 / fblocks) * 8 + (blockIdx.x & 7);
     if (pb >= pblocks) return;  // the whole workgroup
-    const int T0 = 4 * fb;
+    const int T0 = 2 * FW * fb;
 
-    // this wave's four copies of a stage: fragments of weights (waves 0-3), of rows (waves 4-7)
-    const char* src[4];
-    const int step = wave < 4 ? 4096 : 64;
+    // this wave's copies of a stage: the four fragments of a group of features (waves below 2 FW), fragments of
+    // rows (FW 2: four by each of the other waves; FW 4: one by every wave)
+    const char* src[C];
+    const auto row = [&](int frag) {
+        int64_t p = pb * kPoints + frag * 16 + r;
+        if (p >= a.n) p = a.n - 1;
+        if constexpr (Op::kInt8) return (const char*)a.q + p * a.steps * 64 + 16 * g;
+        else return (const char*)a.dz + p * a.lddz * 2 + 16 * g;
+    };
+    const bool has_weights = FW == 4 || wave < 4;
+    const int step = has_weights ? 4096 : 64;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (wave < 4) {
+    for (int i = 0; i < C; ++i) {
+        if (i < 4 && has_weights) {
             const int T = T0 + wave < a.groups ? T0 + wave : a.groups - 1;  // a group behind the last is not stored
-            src[i] = a.frags + (size_t)T * a.frag_steps * 4096 + frag_source<OUT>(i, lane);
+            src[i] = a.frags + (size_t)T * a.frag_steps * 4096 + frag_source<OUT>(i & 3, lane);
         } else {
-            int64_t p = pb * 256 + ((wave - 4) * 4 + i) * 16 + r;
-            if (p >= a.n) p = a.n - 1;
-            if constexpr (Op::kInt8) src[i] = (const char*)a.q + p * a.steps * 64 + 16 * g;
-            else src[i] = (const char*)a.dz + p * a.lddz * 2 + 16 * g;
+            src[i] = row(FW == 4 ? wave : (wave - 4) * 4 + i);
         }
     }
     auto issue = [&](int s) {
-        char* dst = ring + (s % kStreamStages) * kStreamStage + wave * 4096;
+        char* st = ring + (s % S) * kStreamStage<FW>;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) glds16_untracked(src[i] + (int64_t)s * step, dst + i * 1024);
+        for (int i = 0; i < C; ++i)
+            glds16_untracked(src[i] + (int64_t)s * (i < 4 ? step : 64), st + (i < 4 ? wave * 4 + i : 8 * FW + wave) * 1024);
     };
 
     if constexpr (Op::kInt8) {
-        stage_channels(a, ws, bs, 64 * T0, 256);  // read behind the barriers of the loop
+        stage_channels(a, ws, bs, 64 * T0, kFeatures);  // read behind the barriers of the loop
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing but the copies is counted from here on
     }
-    const int wf = wave & 1, wp = wave >> 1;
+    const int wf = wave % FW, wp = wave / FW;
     typename Op::Acc acc[4][2][4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -617,20 +633,20 @@ __global__ __launch_bounds__(kStreamThreads) void linear_streamed_kernel(LinearA
 #pragma unroll
             for (int u = 0; u < 4; ++u) acc[j][t][u] = typename Op::Acc{};
 #pragma unroll
-    for (int s = 0; s < kStreamStages - 1; ++s)
+    for (int s = 0; s < S - 1; ++s)
         if (s < a.steps) issue(s);
     for (int s = 0; s < a.steps; ++s) {
-        // this wave's copies of stage s have arrived (two younger stages of four may be on their way), then everyone's
+        // this wave's copies of stage s have arrived (the younger stages may be on their way), then everyone's
         const int younger = a.steps - 1 - s;
-        if (younger >= 2) wait_vmcnt_n(8);
-        else if (younger == 1) wait_vmcnt_n(4);
+        if (younger >= S - 2) wait_vmcnt_n(C * (S - 2));
+        else if (S > 3 && younger == 1) wait_vmcnt_n(C);
         else wait_vmcnt_n(0);
         // (lgkmcnt: this wave's reads of the stage that is overwritten next have arrived)
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (s + kStreamStages - 1 < a.steps) issue(s + kStreamStages - 1);
-        const char* st = ring + (s % kStreamStages) * kStreamStage + lane * 16;
+        if (s + S - 1 < a.steps) issue(s + S - 1);
+        const char* st = ring + (s % S) * kStreamStage<FW> + lane * 16;
         const char* wl = st + wf * 8 * 1024;
-        const char* xl = st + 16 * 1024 + wp * 4 * 1024;
+        const char* xl = st + 8 * FW * 1024 + wp * 4 * 1024;
         const auto rows = [&](int j) { return typename Op::B(Op::raw_of(*(const i32x4*)(xl + j * 1024))); };
         const typename Op::B b[4] = {rows(0), rows(1), rows(2), rows(3)};
 #pragma unroll
@@ -642,28 +658,91 @@ __global__ __launch_bounds__(kStreamThreads) void linear_streamed_kernel(LinearA
                 for (int j = 0; j < 4; ++j) acc[j][t][u] = Op::mma(wfr, b[j], acc[j][t][u]);
             }
     }
+    const int64_t p0 = pb * kPoints + wp * 64 + r;
+    if constexpr (OUT < TO_INT8) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int64_t p = pb * 256 + (wp * 4 + j) * 16 + r;
-        const bool live = p < a.n;
-        const int64_t pc = live ? p : a.n - 1;
-        float xs = 0.f;
-        if constexpr (Op::kInt8) xs = a.scale[pc];
+        for (int j = 0; j < 4; ++j) {
+            const bool live = p0 + 16 * j < a.n;
+            const int64_t p = live ? p0 + 16 * j : a.n - 1;
+            float xs = 0.f;
+            if constexpr (Op::kInt8) xs = a.scale[p];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int T = 2 * wf + t;
-            const bool whole = 64 * (T0 + T) + 64 <= a.features;
-            if (T0 + T < a.groups) {
-                if constexpr (Op::kInt8) {
-                    float v[16];
-                    finish_linear<OUT, ADD>(a, acc[j][t], ws + 64 * T, bs + 64 * T, xs, 64 * (T0 + T), g, pc, whole, a.relu != 0, v);
-                    if (live) put<OUT>(a, pc, 64 * (T0 + T), g, whole, v);
-                } else if (live) {
-                    const uint2 m = a.mask ? *(const uint2*)(a.mask + pc * (a.groups * 8) + 8 * (T0 + T)) : make_uint2(~0u, ~0u);
-                    put_grad<OUT>(a, acc[j][t], 64 * (T0 + T), g, pc, whole, own_bits<OUT>(m, g));
+            for (int t = 0; t < 2; ++t) {
+                const int T = 2 * wf + t;
+                const bool whole = 64 * (T0 + T) + 64 <= a.features;
+                if (T0 + T < a.groups) {
+                    if constexpr (Op::kInt8) {
+                        float v[16];
+                        finish_linear<OUT, ADD>(a, acc[j][t], ws + 64 * T, bs + 64 * T, xs, 64 * (T0 + T), g, p, whole, a.relu != 0, v);
+                        if (live) put<OUT>(a, p, 64 * (T0 + T), g, whole, v);
+                    } else if (live) {
+                        const uint2 m = a.mask ? *(const uint2*)(a.mask + p * (a.groups * 8) + 8 * (T0 + T)) : make_uint2(~0u, ~0u);
+                        put_grad<OUT>(a, acc[j][t], 64 * (T0 + T), g, p, whole, own_bits<OUT>(m, g));
+                    }
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            __builtin_amdgcn_sched_barrier(0);
+        }
+    } else {
+        // one feature block: the largest of a point's features in this wave, then in all FW that share it
+        constexpr bool RELU = (OUT & 1) != 0, POW2 = (OUT & 2) != 0;
+        float v[4][2][16];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t p = p0 + 16 * j < a.n ? p0 + 16 * j : a.n - 1;
+            const float xs = a.scale[p];
+            unsigned top = 0u;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int T = 2 * wf + t;
+                if (T < a.groups) {  // (an addend's rows are whole groups here)
+                    finish_linear<OUT, ADD>(a, acc[j][t], ws + 64 * T, bs + 64 * T, xs, 64 * T, g, p, true, RELU, v[j][t]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[j][t][i] = 0.f;
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const unsigned m = RELU ? __builtin_bit_cast(unsigned, v[j][t][i]) : magnitude(v[j][t][i]);
+                    top = top > m ? top : m;
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int off = 16; off < 64; off *= 2) {
+                const unsigned o = (unsigned)__shfl_xor((int)top, off);
+                top = top > o ? top : o;
+            }
+            if (g == 0) tops[wf * kPoints + wp * 64 + 16 * j + r] = top;
+        }
+        __syncthreads();
+        const int fp = a.groups * 64;  // width of a row of the output
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t p = p0 + 16 * j;
+            const bool live = p < a.n;
+            unsigned top = 0u;
+#pragma unroll
+            for (int w = 0; w < FW; ++w) {
+                const unsigned o = tops[w * kPoints + wp * 64 + 16 * j + r];
+                top = top > o ? top : o;
+            }
+            const Scale sc = scale_of(top, POW2);
+            const bool has_nan = __any(top > 0x7f800000u);
+            if (live && g == 0 && wf == 0) a.out_scale[p] = sc.scale;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int T = 2 * wf + t;
+                if (T < a.groups) {
+                    const uint4 o = round16<POW2>(v[j][t], sc.inv);
+                    if (live) *(uint4*)((signed char*)a.out + p * fp + 64 * T + 16 * g) = o;
+                    if (a.out_mask) {
+                        const unsigned bits = positive_bits<RELU>(v[j][t], has_nan);
+                        if (live) *(unsigned short*)(a.out_mask + p * (fp / 8) + 8 * T + 2 * g) = (unsigned short)bits;
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     }
 }
@@ -688,16 +767,16 @@ int launch_resident(const LinearArgs& a, const char* what, hipStream_t st) {
     return check_launch(what);
 }
 
-template <class Op, int OUT, int ADD>
+template <class Op, int OUT, int ADD, int FW>
 int launch_streamed(const LinearArgs& a, const char* what, hipStream_t st) {
-    constexpr size_t lds = 2 * 256 * 4 + kStreamStages * kStreamStage;
-    auto kernel = linear_streamed_kernel<Op, OUT, ADD>;
+    static_assert(kStreamLds<FW> <= kLdsBytes, "does not fit");
+    auto kernel = linear_streamed_kernel<Op, OUT, ADD, FW>;
     const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes);
     if (e != hipSuccess) return NERF_FAIL((int)e, "%s: %s", what, hipGetErrorString(e));
-    const int fblocks = (a.groups + 3) / 4;
-    const int64_t pblocks = (a.n + 255) / 256, grid = (pblocks + 7) / 8 * 8 * fblocks;
+    const int fblocks = (a.groups + 2 * FW - 1) / (2 * FW);
+    const int64_t pblocks = (a.n + kStreamPoints<FW> - 1) / kStreamPoints<FW>, grid = (pblocks + 7) / 8 * 8 * fblocks;
     if (grid >= (1LL << 23)) return NERF_FAIL(NERF_E_UNSUPPORTED, "%s: too many rows", what);  // fewer than 2^32 work items
-    kernel<<<(unsigned)grid, kStreamThreads, lds, st>>>(a, fblocks, pblocks);
+    kernel<<<(unsigned)grid, kStreamThreads, kStreamLds<FW>, st>>>(a, fblocks, pblocks);
     return check_launch(what);
 }
 

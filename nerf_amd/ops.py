@@ -595,10 +595,14 @@ def linear_int8(rows, weights, bias=None, relu=False, addend=None, dtype=torch.f
 
 def linear_int8_quantized(rows, weights, bias=None, relu=False, addend=None, pow2=False, want_mask=False):
     """quantize_rows(linear_int8(...), pow2, want_mask), with y in fp32 in between: the next layer's input.  One
-    kernel that never stores y for up to 256 outputs of up to 576 inputs (with an addend a multiple of 64
-    outputs); the two calls otherwise."""
+    kernel that never stores y for up to 512 outputs (with an addend a multiple of 64), but for few rows of many
+    inputs; the two calls otherwise."""
     dev, bias, addend, add_dtype, ldadd = _linear_inputs("linear_int8_quantized", rows, weights, bias, addend)
-    if weights.m > nv.lib().nerf_linear_int8_quantized_width(rows.k) or (addend is not None and weights.m % 64 != 0):
+    # (a row's outputs form in one workgroup: under 4096 rows of over 576 inputs, whose weights are not resident, few
+    # of those run and each waits for one step of inputs after the other.  4000 rows: 1024 x 256 26 us, two calls 18;
+    # 2048 x 512 39, 27; 512 x 512 20, 19.  65536 rows, 1024 x 256: 34 us, two calls 50)
+    if (weights.m > nv.lib().nerf_linear_int8_quantized_width(rows.k) or (addend is not None and weights.m % 64 != 0)
+            or (rows.n < 4096 and rows.k > 576)):
         return quantize_rows(linear_int8(rows, weights, bias, relu, addend), pow2, want_mask)
     n, m = rows.n, weights.m
     q, scale, mask = _new_rows(n, m, dev, want_mask)
