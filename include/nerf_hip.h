@@ -321,12 +321,14 @@ int nerf_linear_int8(const signed char* q, const float* scale, int64_t n, int k,
                      const float* bias, const void* addend, int addend_dtype, int64_t ldadd, int relu,
                      void* y, int dtype, int64_t ldy, nerf_stream_t stream);
 
-/* nerf_quantize_rows of that y (in fp32, never stored): the next layer's rows, yq [n][m rounded up to 64].  For
- * m up to nerf_linear_int8_quantized_width(k) (512), and with an addend m a multiple of 64; otherwise NERF_E_UNSUPPORTED. */
-int nerf_linear_int8_quantized_width(int k);
+/* nerf_quantize_rows of that y (in fp32, never stored): the next layer's rows, yq [n][m rounded up to 64].
+ * With an addend m must be a multiple of 64, otherwise NERF_E_UNSUPPORTED.  workspace:
+ * nerf_linear_int8_quantized_bytes(n, m) bytes (0 up to 512 outputs: NULL will do). */
+size_t nerf_linear_int8_quantized_bytes(int64_t n, int m);
 int nerf_linear_int8_quantized(const signed char* q, const float* scale, int64_t n, int k, const void* packed, int m,
                                const float* bias, const void* addend, int addend_dtype, int64_t ldadd, int relu,
-                               int pow2, signed char* yq, float* yscale, unsigned char* ymask, nerf_stream_t stream);
+                               int pow2, signed char* yq, float* yscale, unsigned char* ymask, void* workspace,
+                               size_t workspace_bytes, nerf_stream_t stream);
 
 /* dx [n][k] = dz [n][m] times the transposed weights as the forward pass used them (packed with pow2 only:
  * they are then exact in bf16), zero where the bit of `mask` is 0.  dz is taken as the exact sum of 1, 2

@@ -54,8 +54,8 @@ SIGNATURES = {
     "nerf_int8_packed_bytes": (_c.c_size_t, [_I, _I, _I]),
     "nerf_int8_pack": (_I, [_P, _I, _I, _I, _P, _P]),
     "nerf_linear_int8": (_I, [_P, _P, _L, _I, _P, _I, _P, _P, _I, _L, _I, _P, _I, _L, _P]),
-    "nerf_linear_int8_quantized_width": (_I, [_I]),
-    "nerf_linear_int8_quantized": (_I, [_P, _P, _L, _I, _P, _I, _P, _P, _I, _L, _I, _I, _P, _P, _P, _P]),
+    "nerf_linear_int8_quantized_bytes": (_c.c_size_t, [_L, _I]),
+    "nerf_linear_int8_quantized": (_I, [_P, _P, _L, _I, _P, _I, _P, _P, _I, _L, _I, _I, _P, _P, _P, _P, _c.c_size_t, _P]),
     "nerf_linear_int8_grad_input": (_I, [_P, _I, _L, _I, _L, _P, _I, _P, _P, _L, _P]),
     "nerf_linear_int8_grad_weight_bytes": (_c.c_size_t, [_L, _I, _I]),
     "nerf_linear_int8_grad_weight": (_I, [_P, _P, _L, _I, _P, _I, _I, _L, _P, _P, _P, _c.c_size_t, _P]),

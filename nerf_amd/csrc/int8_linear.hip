@@ -7,6 +7,9 @@ namespace i8 {
 // Rows from which the resident kernel's copy of the weights into every CU pays.
 constexpr int64_t kResidentRows = 4096;
 
+// Groups of 64 channels up to which a row of 8-bit output is one workgroup's.
+constexpr int kRowGroups = 8;
+
 // Tiles of 16 points a wave works on at a time: two halve the reads of LDS and of the channel scales, where
 // the registers hold the sums of both.
 template <int OUT, int NT, int CH, int ADD>
@@ -34,6 +37,13 @@ static int launch(const LinearArgs& a, const char* what, hipStream_t st) {
         if (!fits) return launch_streamed<Int8Op, OUT, ADD, 2>(a, what, st);
     } else if (!fits) {
         // a whole row in one workgroup (262144 x 512 x 512: 150 us, through an fp32 row and quantize_rows 319)
+        if (a.groups > kRowGroups) {
+            LinearArgs b = a;
+            b.pass = 1;
+            if (int rc = launch_streamed<Int8Op, OUT, ADD, 2>(b, what, st)) return rc;
+            b.pass = 2;
+            return launch_streamed<Int8Op, OUT, ADD, 2>(b, what, st);
+        }
         if (a.groups > 4) return launch_streamed<Int8Op, OUT, ADD, 4>(a, what, st);
         return launch_streamed<Int8Op, OUT, ADD, 2>(a, what, st);
     }
@@ -88,24 +98,28 @@ NERF_API int nerf_linear_int8(const signed char* q, const float* scale, int64_t 
     return launch<NERF_BF16>(a, addend_dtype, what, st);
 }
 
-NERF_API int nerf_linear_int8_quantized_width(int k) {
-    return k >= 1 && k <= kMaxWidth ? 512 : 0;  // all channels of a row in one workgroup
+NERF_API size_t nerf_linear_int8_quantized_bytes(int64_t n, int m) {
+    if (n < 1 || m < 1 || m > kMaxWidth) return 0;
+    const int groups = (int)(up64(m) / 64);
+    return groups > kRowGroups ? (size_t)n * ((groups + 3) / 4) * sizeof(unsigned) : 0;
 }
 
 NERF_API int nerf_linear_int8_quantized(const signed char* q, const float* scale, int64_t n, int k, const void* packed, int m,
                                         const float* bias, const void* addend, int addend_dtype, int64_t ldadd, int relu,
-                                        int pow2, signed char* yq, float* yscale, unsigned char* ymask, nerf_stream_t stream) {
+                                        int pow2, signed char* yq, float* yscale, unsigned char* ymask, void* workspace,
+                                        size_t workspace_bytes, nerf_stream_t stream) {
     const char* what = "nerf_linear_int8_quantized";
     LinearArgs a{};
     if (int rc = linear_args(a, what, q, scale, n, k, packed, m, bias, addend, addend_dtype, ldadd, relu)) return rc;
-    if (m > nerf_linear_int8_quantized_width(k))
-        return NERF_FAIL(NERF_E_UNSUPPORTED, "%s: %d outputs do not fit one workgroup", what, m);
     if (addend && m % 64 != 0)
         return NERF_FAIL(NERF_E_UNSUPPORTED, "%s: an addend of %d columns is not a whole number of 64", what, m);
     if (n == 0) return 0;
     NERF_REQUIRE(yq && yscale, "%s: null pointer", what);
     NERF_REQUIRE(((uintptr_t)yq & 15) == 0 && ((uintptr_t)yscale & 3) == 0 && ((uintptr_t)ymask & 1) == 0, "%s: misaligned pointer", what);
-    a.out = yq, a.out_scale = yscale, a.out_mask = ymask;
+    const size_t need = nerf_linear_int8_quantized_bytes(n, m);
+    NERF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 3) == 0),
+                 "%s: needs a workspace of %zu bytes, got %zu", what, need, workspace ? workspace_bytes : 0);
+    a.out = yq, a.out_scale = yscale, a.out_mask = ymask, a.tops = (unsigned*)workspace;
     hipStream_t st = as_stream(stream);
     if (pow2) return relu ? launch<TO_INT8 + 3>(a, addend_dtype, what, st) : launch<TO_INT8 + 2>(a, addend_dtype, what, st);
     return relu ? launch<TO_INT8 + 1>(a, addend_dtype, what, st) : launch<TO_INT8>(a, addend_dtype, what, st);

@@ -38,6 +38,8 @@ struct LinearArgs {
     // output in 8 bits (TO_INT8): out = integers, and
     float* out_scale;
     unsigned char* out_mask;
+    unsigned* tops;        // of rows beyond one workgroup: [n][feature blocks] largest magnitudes
+    int pass;              // ... 1: they are formed, 2: they are read; 0: a row is one workgroup's
 };
 
 // What a product is stored as: a type (NERF_F32, ...) or 8-bit rows: TO_INT8, + 1 behind a ReLU, + 2 with
@@ -569,7 +571,8 @@ __global__ __launch_bounds__(kResidentThreads) void linear_resident_kernel(Linea
 // which the die's L2 then holds.  Bound by the matrix unit: 32768 x 2048 x 2048 144 us, 1.9 P op/s (weights
 // and rows straight from memory: 253 us).
 // FW 2: tiles of 256 x 256 and four stages of 32 KiB.  FW 4: 512 x 128 and three of 40 KiB, for 8-bit output of
-// more than 256 features, whose scale takes the whole row: the waves' maxima meet in LDS.
+// 257 to 512 features, whose scale takes the whole row: the waves' maxima meet in LDS.  Longer rows with 8-bit
+// output are formed twice, first for their blocks' maxima, then for their integers.
 constexpr int kStreamThreads = 512;
 template <int FW> constexpr int kStreamStages = FW == 2 ? 4 : 3;
 template <int FW> constexpr int kStreamStage = (8 * FW + 32 / FW) * 1024;
@@ -684,7 +687,7 @@ __global__ __launch_bounds__(kStreamThreads) void linear_streamed_kernel(LinearA
             }
         }
     } else {
-        // one feature block: the largest of a point's features in this wave, then in all FW that share it
+        // the largest of a point's features in this wave, in all FW that share it, and in all workgroups
         constexpr bool RELU = (OUT & 1) != 0, POW2 = (OUT & 2) != 0;
         float v[4][2][16];
 #pragma unroll
@@ -695,8 +698,8 @@ __global__ __launch_bounds__(kStreamThreads) void linear_streamed_kernel(LinearA
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const int T = 2 * wf + t;
-                if (T < a.groups) {  // (an addend's rows are whole groups here)
-                    finish_linear<OUT, ADD>(a, acc[j][t], ws + 64 * T, bs + 64 * T, xs, 64 * T, g, p, true, RELU, v[j][t]);
+                if (T0 + T < a.groups) {  // (an addend's rows are whole groups here)
+                    finish_linear<OUT, ADD>(a, acc[j][t], ws + 64 * T, bs + 64 * T, xs, 64 * (T0 + T), g, p, true, RELU, v[j][t]);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) v[j][t][i] = 0.f;
@@ -713,9 +716,25 @@ __global__ __launch_bounds__(kStreamThreads) void linear_streamed_kernel(LinearA
                 const unsigned o = (unsigned)__shfl_xor((int)top, off);
                 top = top > o ? top : o;
             }
-            if (g == 0) tops[wf * kPoints + wp * 64 + 16 * j + r] = top;
+            if (g == 0 && a.pass != 2) tops[wf * kPoints + wp * 64 + 16 * j + r] = top;
+        }
+        if (a.pass == 2) {
+            const int64_t p = pb * kPoints + threadIdx.x % kPoints;
+            unsigned top = 0u;
+            if (p < a.n)
+                for (int i = threadIdx.x / kPoints; i < fblocks; i += FW) top = top > a.tops[p * fblocks + i] ? top : a.tops[p * fblocks + i];
+            tops[threadIdx.x] = top;  // [FW][kPoints]: kStreamThreads
         }
         __syncthreads();
+        if (a.pass == 1) {
+            const int64_t p = pb * kPoints + threadIdx.x;
+            if (threadIdx.x < kPoints && p < a.n) {
+                unsigned top = 0u;
+                for (int w = 0; w < FW; ++w) top = top > tops[w * kPoints + threadIdx.x] ? top : tops[w * kPoints + threadIdx.x];
+                a.tops[p * fblocks + fb] = top;
+            }
+            return;
+        }
         const int fp = a.groups * 64;  // width of a row of the output
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -729,16 +748,16 @@ __global__ __launch_bounds__(kStreamThreads) void linear_streamed_kernel(LinearA
             }
             const Scale sc = scale_of(top, POW2);
             const bool has_nan = __any(top > 0x7f800000u);
-            if (live && g == 0 && wf == 0) a.out_scale[p] = sc.scale;
+            if (live && g == 0 && wf == 0 && fb == 0) a.out_scale[p] = sc.scale;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const int T = 2 * wf + t;
-                if (T < a.groups) {
+                if (T0 + T < a.groups) {
                     const uint4 o = round16<POW2>(v[j][t], sc.inv);
-                    if (live) *(uint4*)((signed char*)a.out + p * fp + 64 * T + 16 * g) = o;
+                    if (live) *(uint4*)((signed char*)a.out + p * fp + 64 * (T0 + T) + 16 * g) = o;
                     if (a.out_mask) {
                         const unsigned bits = positive_bits<RELU>(v[j][t], has_nan);
-                        if (live) *(unsigned short*)(a.out_mask + p * (fp / 8) + 8 * T + 2 * g) = (unsigned short)bits;
+                        if (live) *(unsigned short*)(a.out_mask + p * (fp / 8) + 8 * (T0 + T) + 2 * g) = (unsigned short)bits;
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);
@@ -774,6 +793,7 @@ int launch_streamed(const LinearArgs& a, const char* what, hipStream_t st) {
     const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes);
     if (e != hipSuccess) return NERF_FAIL((int)e, "%s: %s", what, hipGetErrorString(e));
     const int fblocks = (a.groups + 2 * FW - 1) / (2 * FW);
+    static_assert(FW * kStreamPoints<FW> == kStreamThreads, "a thread per maximum");
     const int64_t pblocks = (a.n + kStreamPoints<FW> - 1) / kStreamPoints<FW>, grid = (pblocks + 7) / 8 * 8 * fblocks;
     if (grid >= (1LL << 23)) return NERF_FAIL(NERF_E_UNSUPPORTED, "%s: too many rows", what);  // fewer than 2^32 work items
     kernel<<<(unsigned)grid, kStreamThreads, kStreamLds<FW>, st>>>(a, fblocks, pblocks);

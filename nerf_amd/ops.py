@@ -595,19 +595,23 @@ def linear_int8(rows, weights, bias=None, relu=False, addend=None, dtype=torch.f
 
 def linear_int8_quantized(rows, weights, bias=None, relu=False, addend=None, pow2=False, want_mask=False):
     """quantize_rows(linear_int8(...), pow2, want_mask), with y in fp32 in between: the next layer's input.  One
-    kernel that never stores y for up to 512 outputs (with an addend a multiple of 64), but for few rows of many
-    inputs; the two calls otherwise."""
+    call that never stores y, but where storing it is faster or an addend is not a multiple of 64 wide: the two
+    calls."""
     dev, bias, addend, add_dtype, ldadd = _linear_inputs("linear_int8_quantized", rows, weights, bias, addend)
-    # (a row's outputs form in one workgroup: under 4096 rows of over 576 inputs, whose weights are not resident, few
-    # of those run and each waits for one step of inputs after the other.  4000 rows: 1024 x 256 26 us, two calls 18;
-    # 2048 x 512 39, 27; 512 x 512 20, 19.  65536 rows, 1024 x 256: 34 us, two calls 50)
-    if (weights.m > nv.lib().nerf_linear_int8_quantized_width(rows.k) or (addend is not None and weights.m % 64 != 0)
-            or (rows.n < 4096 and rows.k > 576)):
-        return quantize_rows(linear_int8(rows, weights, bias, relu, addend), pow2, want_mask)
+    # (one call, two calls, us.  Up to 512 outputs a row forms in one workgroup: under 4096 rows of over 576 inputs,
+    # whose weights are not resident, few of those run and each waits for one step of inputs after the other.  4000 rows:
+    # 1024 x 256 26, 18; 2048 x 512 39, 27; 512 x 512 20, 19; 65536 rows, 1024 x 256: 34, 50.  Beyond, the products are
+    # formed twice.  300 rows, 500 x 1000: 32, 17; 162501 rows, 120 x 1271: 218, 437; 32768 rows, 512 x 1024: 65, 73,
+    # 1024 x 1024 89, 85, 2048 x 1024 136, 108)
     n, m = rows.n, weights.m
+    if (addend is not None and m % 64 != 0) or (n < 4096 and (rows.k > 576 or m > 512)) or (rows.k > 1024 and m > 512):
+        return quantize_rows(linear_int8(rows, weights, bias, relu, addend), pow2, want_mask)
     q, scale, mask = _new_rows(n, m, dev, want_mask)
+    need = nv.lib().nerf_linear_int8_quantized_bytes(n, m) if m > 512 else 0
+    ws = _new((need,), torch.uint8, dev) if need else None
     _call("nerf_linear_int8_quantized", dev, rows.q.data_ptr(), rows.scale.data_ptr(), n, rows.k, weights.packed.data_ptr(), m,
-          _addr(bias), _addr(addend), add_dtype, ldadd, 1 if relu else 0, 1 if pow2 else 0, q.data_ptr(), scale.data_ptr(), _addr(mask))
+          _addr(bias), _addr(addend), add_dtype, ldadd, 1 if relu else 0, 1 if pow2 else 0, q.data_ptr(), scale.data_ptr(), _addr(mask),
+          _addr(ws), need)
     return Int8Rows._made(q, scale, m, pow2, mask)
 
 

@@ -15,7 +15,7 @@ TINY = {t: max(torch.finfo(t).smallest_normal * torch.finfo(t).eps, 1e-38) for t
 SHAPES = [(1, 1, 1), (1, 256, 256), (3, 63, 5), (17, 64, 64), (31, 65, 63), (33, 128, 3), (64, 319, 256), (257, 283, 128),
           (1000, 27, 129), (130, 2048, 17), (65, 130, 700), (4100, 256, 256), (129, 600, 1), (16, 2047, 33),
           (4111, 63, 256), (4099, 283, 128), (5003, 319, 256), (4097, 128, 3), (6001, 27, 70), (4133, 700, 200), (4100, 1100, 65), (33000, 256, 192), (70001, 64, 64), (5000, 100, 96), (4200, 640, 600), (4500, 576, 1000), (4300, 1000, 576), (6000, 512, 512), (4200, 832, 190), (4100, 640, 150),
-          (300, 1000, 320), (5000, 40, 400), (9000, 100, 510), (1, 2, 300)]
+          (300, 1000, 320), (5000, 40, 400), (9000, 100, 510), (1, 2, 300), (700, 200, 1344), (1, 65, 513)]
 
 
 # ---- without a GPU -----------------------------------------------------------------------------------
@@ -47,13 +47,15 @@ def test_bad_arguments_are_refused_without_a_gpu():
                 dict(dt=5), dict(ldy=7), dict(addend=one, ldadd=7), dict(addend=one, ldadd=8, adt=9), dict(bias=odd), dict(y=odd)):
         assert linear(**bad) == -1, bad
     assert linear(n=0, q=None) == 0
-    assert lib.nerf_linear_int8_quantized_width(65536) == 512 and lib.nerf_linear_int8_quantized_width(0) == 0
+    size = lib.nerf_linear_int8_quantized_bytes
+    assert size(10, 512) == 0 and size(10, 513) == 10 * 3 * 4 and size(1, 65536) == 256 * 4 and size(0, 600) == 0 and size(5, 65537) == 0
     quant = lambda **c: lib.nerf_linear_int8_quantized(*[{**dict(q=one, scale=one, n=4, k=8, packed=one, m=8, bias=None, addend=None, adt=0, ldadd=0,
-                                                                 relu=0, pow2=0, yq=one, ys=one, ym=None, st=None), **c}[x] for x in
-                                                         ("q", "scale", "n", "k", "packed", "m", "bias", "addend", "adt", "ldadd", "relu", "pow2", "yq", "ys", "ym", "st")])
-    for bad in (dict(q=None), dict(yq=None), dict(ys=None), dict(yq=odd), dict(ym=odd), dict(k=0), dict(m=0), dict(n=-1), dict(addend=one, ldadd=7)):
+                                                                 relu=0, pow2=0, yq=one, ys=one, ym=None, ws=None, size=0, st=None), **c}[x] for x in
+                                                         ("q", "scale", "n", "k", "packed", "m", "bias", "addend", "adt", "ldadd", "relu", "pow2", "yq", "ys", "ym", "ws", "size", "st")])
+    for bad in (dict(q=None), dict(yq=None), dict(ys=None), dict(yq=odd), dict(ym=odd), dict(k=0), dict(m=0), dict(n=-1), dict(addend=one, ldadd=7), dict(m=513), dict(m=513, ws=one, size=47),
+                dict(m=513, ws=odd, size=48)):
         assert quant(**bad) == -1, bad
-    assert quant(m=513) == -2 and quant(m=65, addend=one, ldadd=65) == -2
+    assert quant(m=65, addend=one, ldadd=65) == -2
     assert quant(m=64, addend=one, ldadd=64, adt=1) == -1      # an addend is fp32 or bf16
     gi = lambda **c: lib.nerf_linear_int8_grad_input(*[{**dict(dz=one, dt=0, n=4, m=8, lddz=8, packed=one, k=8, mask=None, dx=one, lddx=8, st=None), **c}[x]
                                                        for x in ("dz", "dt", "n", "m", "lddz", "packed", "k", "mask", "dx", "lddx", "st")])
@@ -388,7 +390,7 @@ def _layer(x, w, dz, b):
 
 
 @gpu_only
-@pytest.mark.parametrize("n,k,m", [(700, 63, 256), (1, 256, 128), (5000, 256, 256), (4500, 320, 384)])
+@pytest.mark.parametrize("n,k,m", [(700, 63, 256), (1, 256, 128), (5000, 256, 256), (4500, 320, 384), (600, 64, 800)])
 def test_a_layer_on_other_streams_and_in_graphs(gpu, n, k, m):
     """Two streams at once, and two captured graphs replayed in turn on fresh inputs, with eager work between:
     the bits of the plain calls."""
@@ -478,7 +480,7 @@ def test_a_row_that_is_not_finite_stays_one_row(gpu, n, k, m, dtype):
 
 @gpu_only
 @pytest.mark.parametrize("dt,t", [(0, torch.float32), (1, torch.float16), (2, torch.bfloat16)])
-@pytest.mark.parametrize("n,k,m", [(1, 5, 3), (37, 70, 19), (4100, 283, 130), (4099, 256, 256), (4100, 65, 600), (4101, 700, 200), (4100, 65, 450), (40, 650, 300), (129, 1000, 70)])
+@pytest.mark.parametrize("n,k,m", [(1, 5, 3), (37, 70, 19), (4100, 283, 130), (4099, 256, 256), (4100, 65, 600), (4101, 700, 200), (4100, 65, 450), (40, 650, 300), (129, 1000, 70), (300, 1100, 1100)])
 def test_nothing_else_is_written(gpu, n, k, m, dt, t):
     """The C entry points on buffers with room between and behind the rows: what is not theirs keeps its bytes."""
     from nerf_amd import _native, ops
@@ -498,13 +500,14 @@ def test_nothing_else_is_written(gpu, n, k, m, dt, t):
                                 y.data_ptr(), dt, m + 5, st) == 0
     assert torch.equal(y[:n, :m], ops.linear_int8(rows, packed, b, relu=True, dtype=t))
     assert bool((y[n:] == 77).all()) and bool((y[:, m:] == 77).all())
-    if m <= 512:
-        yq, ys, yb = fresh(n + 2, mp, torch.int8), fresh(n + 2, 1, torch.float32), fresh(n + 2, mp // 8, torch.uint8)
-        assert lib.nerf_linear_int8_quantized(rows.q.data_ptr(), rows.scale.data_ptr(), n, k, packed.packed.data_ptr(), m, b.data_ptr(), None, 0,
-                                              0, 1, 1, yq.data_ptr(), ys.data_ptr(), yb.data_ptr(), st) == 0
-        ref = ops.linear_int8_quantized(rows, packed, b, relu=True, pow2=True, want_mask=True)
-        assert torch.equal(yq[:n], ref.q) and torch.equal(ys[:n, 0], ref.scale) and torch.equal(yb[:n], ref.mask)
-        assert bool((yq[n:] == 77).all()) and bool((ys[n:] == 77).all()) and bool((yb[n:] == 77).all())
+    need = lib.nerf_linear_int8_quantized_bytes(n, m)
+    ws = fresh(need + 64, 1, torch.uint8)
+    yq, ys, yb = fresh(n + 2, mp, torch.int8), fresh(n + 2, 1, torch.float32), fresh(n + 2, mp // 8, torch.uint8)
+    assert lib.nerf_linear_int8_quantized(rows.q.data_ptr(), rows.scale.data_ptr(), n, k, packed.packed.data_ptr(), m, b.data_ptr(), None, 0,
+                                          0, 1, 1, yq.data_ptr(), ys.data_ptr(), yb.data_ptr(), ws.data_ptr(), need, st) == 0
+    ref = ops.linear_int8_quantized(rows, packed, b, relu=True, pow2=True, want_mask=True)
+    assert torch.equal(yq[:n], ref.q) and torch.equal(ys[:n, 0], ref.scale) and torch.equal(yb[:n], ref.mask)
+    assert bool((yq[n:] == 77).all()) and bool((ys[n:] == 77).all()) and bool((yb[n:] == 77).all()) and bool((ws[need:] == 77).all())
     dx = fresh(n + 2, k + 3, t)
     assert lib.nerf_linear_int8_grad_input(dz.data_ptr(), dt, n, m, m, packed.packed.data_ptr(), k, rows.mask.data_ptr(), dx.data_ptr(), k + 3, st) == 0
     assert torch.equal(dx[:n, :k], ops.linear_int8_grad_input(dz, packed, rows.mask))
