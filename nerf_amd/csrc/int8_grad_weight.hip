@@ -37,22 +37,23 @@ DEV bf16x8 tr_operand(const char* img, int half, int lane) {
     return __builtin_bit_cast(bf16x8, v);
 }
 
-// KT x MT features of dW by four waves, stages of R rows, D of them held ahead in registers (even: the LDS
+// KT x MT features of dW by four waves (256 x 256: eight), stages of R rows, D of them held ahead in registers (even: the LDS
 // buffer of a turn is then known when compiling).
 // EVEN: rows of dz are a whole number of 8-feature pieces, so that every piece is inside its row or wholly
 // behind it (and then any piece of the row will do: its columns are not stored).
 template <int DT, int KT, int MT, int R, int D, bool EVEN>
-__global__ __launch_bounds__(256, 2) void grad_weight_kernel(GradWeightArgs a) {
+__global__ __launch_bounds__(KT == 256 ? 512 : 256, 2) void grad_weight_kernel(GradWeightArgs a) {
+    constexpr int NT = KT == 256 ? 512 : 256;  // threads
     typedef typename Elem<DT>::T T;
     constexpr int N = Terms<DT>::N, YT = MT / 32, XT = KT / 32;
     constexpr int kImg = R * 64;  // bytes of the image of 32 features: [R rows][32 bf16]
     constexpr int kStage = (XT + N * YT) * kImg;
     constexpr int kXPieces = R * KT / 16, kYPieces = R * MT / 8;   // 16 integers, 8 elements of dz
-    constexpr int CX = (kXPieces + 255) / 256, CY = (kYPieces + 255) / 256;  // of a thread
+    constexpr int CX = (kXPieces + NT - 1) / NT, CY = (kYPieces + NT - 1) / NT;  // of a thread
     // waves along k and m, and 32 x 32 tiles of a wave
-    constexpr int WX = MT == 32 ? 4 : KT == 128 ? 2 : 1, WY = 4 / WX, AX = XT / WX, AY = YT / WY;
-    constexpr int kRowBits = R == 64 ? 6 : 5, kTileBits = KT == 128 ? 2 : 1;
-    static_assert((R == 32 || R == 64) && (KT == 64 || KT == 128) && AX >= 1 && AY >= 1 && D % 2 == 0, "shapes");
+    constexpr int WX = MT == 32 ? 4 : KT >= 128 ? 2 : 1, WY = NT / 64 / WX, AX = XT / WX, AY = YT / WY;
+    constexpr int kRowBits = R == 64 ? 6 : 5, kTileBits = KT == 256 ? 3 : KT == 128 ? 2 : 1;
+    static_assert((R == 32 || R == 64) && (KT == 64 || KT == 128 || KT == 256) && AX >= 1 && AY >= 1 && D % 2 == 0, "shapes");
     __shared__ __attribute__((aligned(16))) char lds[2 * kStage];
     static_assert(2 * kStage >= R * MT * 4, "the sums of dz meet in LDS");
 
@@ -77,7 +78,7 @@ __global__ __launch_bounds__(256, 2) void grad_weight_kernel(GradWeightArgs a) {
     auto y_row = [&](int e) { return (e >> 2) & (R - 1); };
     auto y_img = [&](int e) { return e >> (2 + kRowBits); };
     const int yq = t & 3;
-    const bool has_x = kXPieces >= 256 || t < kXPieces, has_y = kYPieces >= 256 || t < kYPieces;
+    const bool has_x = kXPieces >= NT || t < kXPieces, has_y = kYPieces >= NT || t < kYPieces;
     const bool y_whole = mb * MT + MT <= a.m;
 
     struct Held {
@@ -98,16 +99,16 @@ __global__ __launch_bounds__(256, 2) void grad_weight_kernel(GradWeightArgs a) {
     int64_t y_at[CY];
 #pragma unroll
     for (int i = 0; i < CX; ++i) {
-        const int e = t + 256 * i, col = kb * KT + x_img(e) * 32 + x_half(e) * 16;
+        const int e = t + NT * i, col = kb * KT + x_img(e) * 32 + x_half(e) * 16;
         x_at[i] = (unsigned)x_row(e) * a.kp + (col < a.kp ? col : 0);  // (behind the last column: not stored)
         s_at[i] = x_row(e);
     }
     auto y_col = [&](int i) {
-        const int col = mb * MT + y_img(t + 256 * i) * 32 + yq * 8;
+        const int col = mb * MT + y_img(t + NT * i) * 32 + yq * 8;
         return EVEN && col >= a.m ? 0 : col;
     };
 #pragma unroll
-    for (int i = 0; i < CY; ++i) y_at[i] = y_row(t + 256 * i) * a.lddz;
+    for (int i = 0; i < CY; ++i) y_at[i] = y_row(t + NT * i) * a.lddz;
     // the stage from row0, which has rows at least up to row0 + `most`; rows behind repeat that one
     auto fetch = [&](int64_t row0, int most, Held& h) {
         if (has_x) {
@@ -124,7 +125,7 @@ __global__ __launch_bounds__(256, 2) void grad_weight_kernel(GradWeightArgs a) {
             const T* y = (const T*)a.dz + row0 * a.lddz;
 #pragma unroll
             for (int i = 0; i < CY; ++i) {
-                const int row = y_row(t + 256 * i);
+                const int row = y_row(t + NT * i);
                 const T* src = y + (y_at[i] - (row > most ? (row - most) * a.lddz : 0));
                 h.y[i] = load8<T>(src, y_col(i), a.m, EVEN || y_whole);
             }
@@ -135,7 +136,7 @@ __global__ __launch_bounds__(256, 2) void grad_weight_kernel(GradWeightArgs a) {
         if (has_x) {
 #pragma unroll
             for (int i = 0; i < CX; ++i) {
-                const int e = t + 256 * i;
+                const int e = t + NT * i;
                 const float xs = x_row(e) < rows ? h.s[i] : 0.f;
                 bf16x8 o[2];
 #pragma unroll
@@ -150,7 +151,7 @@ __global__ __launch_bounds__(256, 2) void grad_weight_kernel(GradWeightArgs a) {
         if (has_y) {
 #pragma unroll
             for (int i = 0; i < CY; ++i) {
-                const int e = t + 256 * i;
+                const int e = t + NT * i;
                 const bool on = y_row(e) < rows;
                 bf16x8 o[N];
                 if (DT != NERF_BF16 || kb == 0) {
@@ -191,21 +192,32 @@ __global__ __launch_bounds__(256, 2) void grad_weight_kernel(GradWeightArgs a) {
 #pragma unroll
             for (int y = 0; y < AY; ++y) o.y[s][y] = tr_operand(buf + (XT + s * YT + wy + y) * kImg, half, lane);
     };
+    auto products = [&](const Operands& c) {
+#pragma unroll
+        for (int s = 0; s < N; ++s)
+#pragma unroll
+            for (int y = 0; y < AY; ++y)
+#pragma unroll
+                for (int x = 0; x < AX; ++x) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(c.x[x], c.y[s][y], acc[x][y], 0, 0, 0);
+    };
     auto multiply = [&](const char* buf) {
-        Operands o[2];
-        read(buf, 0, o[0]);
+        if constexpr (KT == 256) {  // (no room for two sets)
 #pragma unroll
-        for (int half = 0; half < R / 16; ++half) {
-            if (half + 1 < R / 16) read(buf, half + 1, o[(half + 1) & 1]);
-            __builtin_amdgcn_sched_barrier(0);
-            const Operands& c = o[half & 1];
+            for (int half = 0; half < R / 16; ++half) {
+                Operands o;
+                read(buf, half, o);
+                products(o);
+            }
+        } else {
+            Operands o[2];
+            read(buf, 0, o[0]);
 #pragma unroll
-            for (int s = 0; s < N; ++s)
-#pragma unroll
-                for (int y = 0; y < AY; ++y)
-#pragma unroll
-                    for (int x = 0; x < AX; ++x) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(c.x[x], c.y[s][y], acc[x][y], 0, 0, 0);
-            __builtin_amdgcn_sched_barrier(0);
+            for (int half = 0; half < R / 16; ++half) {
+                if (half + 1 < R / 16) read(buf, half + 1, o[(half + 1) & 1]);
+                __builtin_amdgcn_sched_barrier(0);
+                products(o[half & 1]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     };
     // every fetch is made, also of stages that do not exist (they repeat the last): a wait for older loads
@@ -255,7 +267,7 @@ __global__ __launch_bounds__(256, 2) void grad_weight_kernel(GradWeightArgs a) {
     if (has_y) {
 #pragma unroll
         for (int i = 0; i < CY; ++i) {
-            const int e = t + 256 * i;
+            const int e = t + NT * i;
 #pragma unroll
             for (int j = 0; j < 8; ++j) red[y_row(e) * MT + y_img(e) * 32 + yq * 8 + j] = sum[i][j];
         }
@@ -373,19 +385,26 @@ __global__ __launch_bounds__(256) void grad_weight_join_kernel(const float* __re
 }
 
 // Which tiles, and how the rows are cut: up to `target` workgroups over all tiles, slices of at least 256 rows.
+// bf16 tiles of 256 x 256, one workgroup a CU, read every row once (of 128 x 128: from L2 by two workgroups), but
+// leave twice the partial sums to join.  They are taken where they waste no more than those of 128 and where
+// slices have 2048 rows or more: 786432 x 256 x 256 133 + 11 us (of 128: 144 + 6; memory at the rate of a copy),
+// 262144 x 512 x 256 100 us in all (104), 65536 x 256 x 256 41 us (32).
 struct Cut {
     int tile_k, tile_m;  // tile_m 0: the kernel for few outputs
     int kblocks, mblocks, slices;
     int64_t rows_per;
 };
-static Cut cut_rows(int64_t n, int k, int m) {
+static Cut cut_rows(int64_t n, int k, int m, bool bf16) {
     Cut c;
     const bool thin = m <= 4;
-    c.tile_m = thin ? 0 : m <= 32 ? 32 : 128;
-    c.tile_k = thin ? kThinPieces * 16 : (m > 32 && k <= 64) ? 64 : 128;
-    c.kblocks = (k + c.tile_k - 1) / c.tile_k, c.mblocks = thin ? 1 : (m + c.tile_m - 1) / c.tile_m;
+    const auto blocks_of = [](int size, int tile) { return (size + tile - 1) / tile; };
+    const int k256 = blocks_of(k, 256), m256 = blocks_of(m, 256);
+    const bool wide = bf16 && m % 8 == 0 && 2 * k256 == blocks_of(k, 128) && 2 * m256 == blocks_of(m, 128) && n * k256 * m256 >= 256 * 2048;
+    c.tile_m = thin ? 0 : m <= 32 ? 32 : wide ? 256 : 128;
+    c.tile_k = thin ? kThinPieces * 16 : wide ? 256 : (m > 32 && k <= 64) ? 64 : 128;
+    c.kblocks = blocks_of(k, c.tile_k), c.mblocks = thin ? 1 : blocks_of(m, c.tile_m);
     const int64_t blocks = (int64_t)c.kblocks * c.mblocks;
-    const int64_t target = c.tile_m == 128 ? 512 : 1024;  // two or more workgroups a CU, as their registers allow
+    const int64_t target = wide ? 256 : c.tile_m == 128 ? 512 : 1024;  // as many a CU as their registers allow
     int64_t s = target / blocks;
     const int64_t most = (n + 255) / 256;
     if (s > most) s = most;
@@ -409,7 +428,8 @@ static void launch_grad_weight(const GradWeightArgs& a, const Cut& c, hipStream_
     const unsigned grid = (unsigned)((int64_t)c.kblocks * c.mblocks * c.slices);
     constexpr int D = DT == NERF_F32 ? 2 : 4;
     const bool even = a.m % 8 == 0;
-    if (c.tile_m == 32) grad_weight_kernel<DT, 128, 32, 32, 4, false><<<grid, 256, 0, st>>>(a);
+    if (c.tile_m == 256) grad_weight_kernel<NERF_BF16, 256, 256, 32, 4, true><<<grid, 512, 0, st>>>(a);
+    else if (c.tile_m == 32) grad_weight_kernel<DT, 128, 32, 32, 4, false><<<grid, 256, 0, st>>>(a);
     else if (c.tile_k == 64) {
         if (even) grad_weight_kernel<DT, 64, 128, 32, D, true><<<grid, 256, 0, st>>>(a);
         else grad_weight_kernel<DT, 64, 128, 32, D, false><<<grid, 256, 0, st>>>(a);
@@ -429,8 +449,8 @@ using namespace nerf::i8;
 
 NERF_API size_t nerf_linear_int8_grad_weight_bytes(int64_t n, int k, int m) {
     if (n < 1 || k < 1 || m < 1 || k > kMaxWidth || m > kMaxWidth) return 0;
-    const Cut c = cut_rows(n, k, m);
-    return c.slices > 1 ? (size_t)c.slices * ((size_t)k + 1) * m * sizeof(float) : 0;
+    const int s = cut_rows(n, k, m, false).slices, t = cut_rows(n, k, m, true).slices, slices = s > t ? s : t;
+    return slices > 1 ? (size_t)slices * ((size_t)k + 1) * m * sizeof(float) : 0;
 }
 
 NERF_API int nerf_linear_int8_grad_weight(const signed char* q, const float* scale, int64_t n, int k, const void* dz,
@@ -444,7 +464,7 @@ NERF_API int nerf_linear_int8_grad_weight(const signed char* q, const float* sca
     NERF_REQUIRE(((uintptr_t)q & 15) == 0 && ((uintptr_t)dz & (dtype_size(dtype) - 1)) == 0 &&
                      (((uintptr_t)scale | (uintptr_t)dw | (uintptr_t)db | (uintptr_t)workspace) & 3) == 0,
                  "%s: misaligned pointer", what);
-    const Cut c = cut_rows(n, k, m);
+    const Cut c = cut_rows(n, k, m, dtype == NERF_BF16);
     const size_t need = nerf_linear_int8_grad_weight_bytes(n, k, m);
     NERF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "%s: needs a workspace of %zu bytes, got %zu", what, need, workspace ? workspace_bytes : 0);
     GradWeightArgs a{};

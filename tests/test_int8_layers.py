@@ -15,7 +15,7 @@ TINY = {t: max(torch.finfo(t).smallest_normal * torch.finfo(t).eps, 1e-38) for t
 SHAPES = [(1, 1, 1), (1, 256, 256), (3, 63, 5), (17, 64, 64), (31, 65, 63), (33, 128, 3), (64, 319, 256), (257, 283, 128),
           (1000, 27, 129), (130, 2048, 17), (65, 130, 700), (4100, 256, 256), (129, 600, 1), (16, 2047, 33),
           (4111, 63, 256), (4099, 283, 128), (5003, 319, 256), (4097, 128, 3), (6001, 27, 70), (4133, 700, 200), (4100, 1100, 65), (33000, 256, 192), (70001, 64, 64), (5000, 100, 96), (4200, 640, 600), (4500, 576, 1000), (4300, 1000, 576), (6000, 512, 512), (4200, 832, 190), (4100, 640, 150),
-          (300, 1000, 320), (5000, 40, 400), (9000, 100, 510), (1, 2, 300), (700, 200, 1344), (1, 65, 513)]
+          (300, 1000, 320), (5000, 40, 400), (9000, 100, 510), (1, 2, 300), (700, 200, 1344), (1, 65, 513), (70001, 1024, 512), (524817, 250, 200)]
 
 
 # ---- without a GPU -----------------------------------------------------------------------------------
