@@ -4,8 +4,6 @@
 namespace nerf {
 namespace i8 {
 
-constexpr int64_t kResidentRows = 4096;
-
 // Steps of dz rows in a unit: 256 columns of 16-bit types, 128 of fp32 (32 registers).
 template <int DT> constexpr int kHeld = DT == NERF_F32 ? 4 : 8;
 
@@ -19,11 +17,12 @@ static int resident(const LinearArgs& a, const char* what, hipStream_t st) {
 template <int DT>
 static int launch(const LinearArgs& a, const char* what, hipStream_t st) {
     const int nt = resident_groups(a);
+    // (fp16 and fp32 rows cannot go to LDS as they are: their terms are formed in registers)
+    const bool streamed = DT == NERF_BF16 && (nt == 0 || a.groups > nt) && a.width % 32 == 0 && a.lddz % 8 == 0 && ((uintptr_t)a.dz & 15) == 0;
+    if (few_rows(a, streamed) || (nt == 0 && !streamed)) return launch_direct<Bf16Op<DT, false>, DT, NO_ADD>(a, what, st);
     if constexpr (DT == NERF_BF16) {
-        if (a.n >= kResidentRows && (nt == 0 || a.groups > nt) && a.width % 32 == 0 && a.lddz % 8 == 0 && ((uintptr_t)a.dz & 15) == 0)
-            return launch_streamed<Bf16Op<DT, true>, DT, NO_ADD, 2>(a, what, st);
+        if (streamed) return launch_streamed<Bf16Op<DT, true>, DT, NO_ADD, 2>(a, what, st);
     }
-    if (a.n < kResidentRows || nt == 0) return launch_direct<Bf16Op<DT, false>, DT, NO_ADD>(a, what, st);
     if (nt == 4) return resident<DT, 4>(a, what, st);
     if (nt == 3) return resident<DT, 3>(a, what, st);
     if (nt == 2) return resident<DT, 2>(a, what, st);

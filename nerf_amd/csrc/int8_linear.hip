@@ -4,9 +4,6 @@
 namespace nerf {
 namespace i8 {
 
-// Rows from which the resident kernel's copy of the weights into every CU pays.
-constexpr int64_t kResidentRows = 4096;
-
 // Groups of 64 channels up to which a row of 8-bit output is one workgroup's.
 constexpr int kRowGroups = 8;
 
@@ -33,7 +30,7 @@ static int launch(const LinearArgs& a, const char* what, hipStream_t st) {
     const int nt = a.groups == 3 ? 4 : a.groups;  // (of three groups' kernel one would be idle)
     const bool fits = nt <= 4 && channel_bytes<4>() + (int64_t)nt * a.steps * 4096 <= kLdsBytes;
     if constexpr (OUT < TO_INT8) {
-        if (a.n < kResidentRows) return launch_direct<Int8Op, OUT, ADD>(a, what, st);
+        if (few_rows(a, !fits)) return launch_direct<Int8Op, OUT, ADD>(a, what, st);
         if (!fits) return launch_streamed<Int8Op, OUT, ADD, 2>(a, what, st);
     } else if (!fits) {
         // a whole row in one workgroup (262144 x 512 x 512: 150 us, through an fp32 row and quantize_rows 319)

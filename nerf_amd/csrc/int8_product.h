@@ -813,6 +813,16 @@ inline int require_widths(const char* what, int64_t n, int k, int m) {
     return 0;
 }
 
+// Few enough rows for the direct kernel, whose time goes with its work (each wave reads its rows' and features'
+// operands again) where the others begin with a copy of weights per CU or a tile of 256 points.  us, direct and
+// resident: 256 x 256 to bf16, 4096 rows 4.5, 10.3, 16384 rows 6.9, 11.1, 32768 rows 11.1, 11.8, 65536 rows 18.7,
+// 13.7; 63 x 256 at 32768 and 65536 rows 7.3, 9.0 and 11.6, 10.7; bf16 gradient of 256 x 256 at 16384 rows 9.4, 10.0, at
+// 32768 16.9, 11.0.  Direct and streamed: 512 x 512, 8192 rows 9.3, 14.2, 16384 rows 16.6, 16.1; 1024 x 1024, 4096
+// rows 14.9, 20.0, 8192 rows 26.9, 21.9; bf16 gradient of 512 x 512, 8192 rows 14.6, 19.9, 16384 rows 27.4, 21.4.
+inline bool few_rows(const LinearArgs& a, bool streamed) {
+    return a.n < 32768 && a.n * a.groups * a.steps < (streamed ? 1 << 20 : 1 << 19);
+}
+
 // Groups of features a workgroup of the resident kernel holds: as few feature blocks as LDS allows (each
 // reads the rows again), the groups spread evenly over them (5 groups as 3 + 2 and not 4 + 1: every block
 // gets the same share of the CUs); 0: not even one group fits.

@@ -598,13 +598,13 @@ def linear_int8_quantized(rows, weights, bias=None, relu=False, addend=None, pow
     call that never stores y, but where storing it is faster or an addend is not a multiple of 64 wide: the two
     calls."""
     dev, bias, addend, add_dtype, ldadd = _linear_inputs("linear_int8_quantized", rows, weights, bias, addend)
-    # (one call, two calls, us.  Up to 512 outputs a row forms in one workgroup: under 4096 rows of over 576 inputs,
-    # whose weights are not resident, few of those run and each waits for one step of inputs after the other.  4000 rows:
-    # 1024 x 256 26, 18; 2048 x 512 39, 27; 512 x 512 20, 19; 65536 rows, 1024 x 256: 34, 50.  Beyond, the products are
-    # formed twice.  300 rows, 500 x 1000: 32, 17; 162501 rows, 120 x 1271: 218, 437; 32768 rows, 512 x 1024: 65, 73,
-    # 1024 x 1024 89, 85, 2048 x 1024 136, 108)
+    # (one call, two calls, us.  Up to 512 outputs a row forms in one workgroup: with few rows of over 576 inputs,
+    # whose weights are not resident, few of those run and each waits for one step of inputs after the other.  1024 x 256,
+    # 8192 rows 21, 15, 16384 rows 21, 35; 512 x 512, 4096 rows 15, 14, 16384 rows 16, 31.  Beyond, the products are formed
+    # twice.  500 x 1000, 300 rows 32, 17; 256 x 1024, 8192 rows 22, 29; 32768 rows, 512 x 1024 65, 73, 1024 x 1024 89,
+    # 85, 2048 x 1024 136, 108; 120 x 1271, 162501 rows 218, 437)
     n, m = rows.n, weights.m
-    if (addend is not None and m % 64 != 0) or (n < 4096 and (rows.k > 576 or m > 512)) or (rows.k > 1024 and m > 512):
+    if (addend is not None and m % 64 != 0) or (rows.k > 576 and n < 12288) or (m > 512 and (n < 4096 or rows.k > 1024)):
         return quantize_rows(linear_int8(rows, weights, bias, relu, addend), pow2, want_mask)
     q, scale, mask = _new_rows(n, m, dev, want_mask)
     need = nv.lib().nerf_linear_int8_quantized_bytes(n, m) if m > 512 else 0

@@ -15,7 +15,9 @@ TINY = {t: max(torch.finfo(t).smallest_normal * torch.finfo(t).eps, 1e-38) for t
 SHAPES = [(1, 1, 1), (1, 256, 256), (3, 63, 5), (17, 64, 64), (31, 65, 63), (33, 128, 3), (64, 319, 256), (257, 283, 128),
           (1000, 27, 129), (130, 2048, 17), (65, 130, 700), (4100, 256, 256), (129, 600, 1), (16, 2047, 33),
           (4111, 63, 256), (4099, 283, 128), (5003, 319, 256), (4097, 128, 3), (6001, 27, 70), (4133, 700, 200), (4100, 1100, 65), (33000, 256, 192), (70001, 64, 64), (5000, 100, 96), (4200, 640, 600), (4500, 576, 1000), (4300, 1000, 576), (6000, 512, 512), (4200, 832, 190), (4100, 640, 150),
-          (300, 1000, 320), (5000, 40, 400), (9000, 100, 510), (1, 2, 300), (700, 200, 1344), (1, 65, 513), (70001, 1024, 512), (524817, 250, 200)]
+          (300, 1000, 320), (5000, 40, 400), (9000, 100, 510), (1, 2, 300), (700, 200, 1344), (1, 65, 513), (70001, 1024, 512), (524817, 250, 200),
+          (32801, 63, 256), (32771, 283, 128), (32800, 319, 256), (32770, 128, 3), (33001, 27, 70), (32777, 100, 96), (32773, 832, 190),
+          (32800, 640, 150), (32769, 1, 1), (40001, 576, 130), (4111, 1100, 1100), (9000, 700, 704), (16500, 512, 512), (16501, 96, 576)]
 
 
 # ---- without a GPU -----------------------------------------------------------------------------------
@@ -390,7 +392,7 @@ def _layer(x, w, dz, b):
 
 
 @gpu_only
-@pytest.mark.parametrize("n,k,m", [(700, 63, 256), (1, 256, 128), (5000, 256, 256), (4500, 320, 384), (600, 64, 800)])
+@pytest.mark.parametrize("n,k,m", [(700, 63, 256), (1, 256, 128), (5000, 256, 256), (4500, 320, 384), (600, 64, 800), (33000, 256, 256), (16400, 512, 512)])
 def test_a_layer_on_other_streams_and_in_graphs(gpu, n, k, m):
     """Two streams at once, and two captured graphs replayed in turn on fresh inputs, with eager work between:
     the bits of the plain calls."""
@@ -460,7 +462,8 @@ def test_offsets_beyond_32_bits(gpu):
 
 @gpu_only
 @pytest.mark.parametrize("dtype", list(TYPES))
-@pytest.mark.parametrize("n,k,m", [(40, 70, 96), (5000, 100, 96), (4500, 130, 33), (4200, 64, 3), (4200, 300, 222), (4096, 256, 256), (4300, 640, 600), (4300, 640, 500), (4300, 640, 190)])
+@pytest.mark.parametrize("n,k,m", [(40, 70, 96), (5000, 100, 96), (4500, 130, 33), (4200, 64, 3), (4200, 300, 222), (4096, 256, 256), (4300, 640, 600), (4300, 640, 500), (4300, 640, 190),
+                                   (32900, 300, 222), (33000, 64, 3), (32768, 256, 256), (33000, 130, 33), (16000, 640, 600)])
 def test_a_row_that_is_not_finite_stays_one_row(gpu, n, k, m, dtype):
     """A NaN in one row (in the middle, in the last) reaches that row's results and no other's, whatever the
     width the rows are padded to."""
@@ -480,7 +483,8 @@ def test_a_row_that_is_not_finite_stays_one_row(gpu, n, k, m, dtype):
 
 @gpu_only
 @pytest.mark.parametrize("dt,t", [(0, torch.float32), (1, torch.float16), (2, torch.bfloat16)])
-@pytest.mark.parametrize("n,k,m", [(1, 5, 3), (37, 70, 19), (4100, 283, 130), (4099, 256, 256), (4100, 65, 600), (4101, 700, 200), (4100, 65, 450), (40, 650, 300), (129, 1000, 70), (300, 1100, 1100)])
+@pytest.mark.parametrize("n,k,m", [(1, 5, 3), (37, 70, 19), (4100, 283, 130), (4099, 256, 256), (4100, 65, 600), (4101, 700, 200), (4100, 65, 450), (40, 650, 300), (129, 1000, 70), (300, 1100, 1100),
+                                   (32769, 283, 130), (32801, 256, 256), (33000, 65, 600), (33001, 700, 200)])
 def test_nothing_else_is_written(gpu, n, k, m, dt, t):
     """The C entry points on buffers with room between and behind the rows: what is not theirs keeps its bytes."""
     from nerf_amd import _native, ops
