@@ -505,18 +505,33 @@ class GraphedTrainStep:
         new = lambda: torch.zeros((int(n_rays), 3), dtype=torch.float32, device=dev)
         self.rays, self.target = (new(), new()), new()
         self.captures = 0
-        self.graph = self.out = self._targets = None
+        self.graph = self.out = self._targets = self._leaves = None
 
     def _fwd_bwd(self):
         with GradientTape() as tape:
             rgb, disp, acc, extras = self.render_fn(self.rays)
             loss, _, _, psnr, psnr0 = photometric_loss(rgb, extras.get('rgb0'), self.target)
-        return loss, psnr, psnr0, tape.gradient(loss, self.grad_vars)
+        return loss, psnr, psnr0, tape.gradient(loss, self._leaves)
 
     def _capture(self):
-        # (the parameters' gradient-accumulation nodes were made on whatever stream first used the
-        # parameters; tape.gradient never accumulates into them, so torch's warning about their
-        # stream does not apply here)
+        # The networks are captured on leaves of their own over the same memory: a parameter's
+        # gradient node lives as long as any graph that holds it and belongs to the stream of that
+        # graph, and autograd waits for it at the end of a backward pass, which a capture does not
+        # survive when the stream is another one (the outputs of an eager tape still at hand).
+        held = [m.params for m in self.models]
+        leaf = {id(p): p.detach().requires_grad_(True) for ps in held for p in ps}
+        self._leaves = [leaf.get(id(v), v) for v in self.grad_vars]
+        for m in self.models:
+            m.params = [leaf[id(p)] for p in m.params]
+        try:
+            self._capture_on_leaves()
+        finally:
+            for m, ps in zip(self.models, held):
+                m.params = ps
+
+    def _capture_on_leaves(self):
+        # (torch's warning about the stream of gradient nodes does not apply: tape.gradient never
+        # accumulates into them)
         warn = getattr(torch.autograd.graph, 'set_warn_on_accumulate_grad_stream_mismatch', None)
         if warn is not None:
             warn(False)

@@ -207,6 +207,36 @@ def test_train_steps_plain_and_graphed(gpu):
 
 
 @gpu_only
+@pytest.mark.parametrize("precision", ['int8', None])
+def test_a_step_captured_while_an_eager_graph_lives(gpu, precision):
+    """The outputs of an eager tape over the same parameters, still held, do not disturb a capture: its leaves are its own."""
+    from nerf_amd import training
+    from nerf_amd.run_nerf import create_nerf, render
+    runs = []
+    for graphed in (False, True):
+        torch.manual_seed(4)
+        a = _args() if precision else default_args()
+        a.precision, a.N_samples, a.N_importance, a.no_reload = precision, 12, 9, True
+        kw_train, _, _, grad_vars, models = create_nerf(a)
+        kw_train['perturb'] = 0.
+        nets = [models['model'], models['model_fine']]
+        opt = training.Adam(5e-4).bind_models(nets)
+        fn = lambda r: render(8, 8, 9.0, chunk=1024, rays=r, near=2., far=6., retraw=True, **kw_train)
+        g = torch.Generator(device=gpu).manual_seed(6)
+        o = torch.nn.functional.normalize(torch.randn((32, 3), generator=g, device=gpu), dim=1) * 4
+        t = torch.rand((32, 3), generator=g, device=gpu)
+        with training.GradientTape():
+            held = fn((o, -o / 4))                   # ... and its graph with it
+        params = [list(n.params) for n in nets]
+        step = training.GraphedTrainStep(fn, 32, grad_vars, opt, nets) if graphed else None
+        for _ in range(3):
+            step((o, -o / 4), t) if graphed else training.train_step(fn, (o, -o / 4), t, grad_vars, opt)
+        assert all(p is q for n, ps in zip(nets, params) for p, q in zip(n.params, ps)) and held[0].grad_fn is not None
+        runs.append([n.flat.detach().clone() for n in nets])
+    assert all(torch.equal(x, y) for x, y in zip(*runs))
+
+
+@gpu_only
 def test_two_queries_of_one_network_and_unused_ones(gpu):
     """The coarse network doing the fine pass too: autograd adds both contributions; an output that does not
     reach the loss costs nothing."""
