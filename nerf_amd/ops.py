@@ -506,7 +506,10 @@ class Int8Weights:
     __slots__ = ("packed", "k", "m", "pow2")
 
     def __init__(self, packed, k, m, pow2):
-        self.packed, self.k, self.m, self.pow2 = packed, k, m, pow2
+        need = nv.lib().nerf_int8_packed_bytes(int(k), int(m), 1 if pow2 else 0)
+        if need == 0 or packed.dtype != torch.uint8 or tuple(packed.shape) != (need,) or not packed.is_contiguous():
+            raise ValueError(f"Int8Weights: packed must be {need} contiguous bytes for {k} x {m}, got {packed.dtype} {tuple(packed.shape)}")
+        self.packed, self.k, self.m, self.pow2 = packed, int(k), int(m), bool(pow2)
 
     def __repr__(self):
         return f"Int8Weights(k={self.k}, m={self.m}, pow2={self.pow2})"

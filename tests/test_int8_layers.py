@@ -80,6 +80,17 @@ def test_no_cpu_fallback():
             call()
 
 
+def test_packed_weights_of_another_size_are_refused():
+    from nerf_amd import _native, ops
+    need = _native.lib().nerf_int8_packed_bytes(70, 5, 1)
+    assert ops.Int8Weights(torch.zeros(need, dtype=torch.uint8), 70, 5, True).m == 5
+    for packed, k, m, pow2 in ((torch.zeros(need - 1, dtype=torch.uint8), 70, 5, True), (torch.zeros(need, dtype=torch.uint8), 70, 5, False),
+                               (torch.zeros(need, dtype=torch.int8), 70, 5, True), (torch.zeros(2 * need, dtype=torch.uint8)[::2], 70, 5, True),
+                               (torch.zeros(0, dtype=torch.uint8), 0, 5, True)):
+        with pytest.raises(ValueError):
+            ops.Int8Weights(packed, k, m, pow2)
+
+
 # ---- plain forms ---------------------------------------------------------------------------------------
 def ref_scale(top, pow2):
     """Scales of float32 magnitudes, in float64."""
