@@ -1,4 +1,4 @@
-// Pieces shared by the 8-bit dense-layer kernels (int8_quantize.hip, int8_linear.hip,
+// Pieces shared by the 8-bit dense-layer kernels (int8_quantize.hip, int8_product.h, int8_linear.hip, int8_grad_input.hip,
 // int8_grad_weight.hip): number formats, the layout of packed weights, loads and stores of rows of any type
 // and alignment.
 //
@@ -12,8 +12,9 @@
 //                                              bf16: 7 bits), A operands of v_mfma_f32_16x16x32_bf16
 // A fragment is 1 KiB: lane = row (16 output features) + 16 x piece of the contraction (16 integers or
 // 8 bf16).  Row r of fragment u of a group of 64 features is feature 16 (r >> 2) + 4 u + (r & 3) of
-// the group: the accumulators of a lane (point = lane & 15, g = lane >> 4) over the four fragments are
-// then features 16 g .. 16 g + 15, 16 neighbours in memory, whatever the type that is stored.
+// the group: read as stored, a lane's accumulators (point = lane & 15, g = lane >> 4) over the four fragments
+// are features 16 g .. 16 g + 15, what an 8-bit output stores; for wider types the products read the rows in
+// the order that leaves a lane pieces of 16 bytes.
 #pragma once
 #include "common.h"
 
@@ -25,9 +26,7 @@ namespace i8 {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 __host__ __device__ inline int64_t up64(int64_t v) { return (v + 63) / 64 * 64; }
 

@@ -305,7 +305,7 @@ __global__ __launch_bounds__(256) void grad_weight_thin_kernel(GradWeightArgs a)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[j][i] = 0.f;
     }
-    constexpr int U = 4;  // rows of a thread on their way at a time
+    constexpr int U = 8;  // rows of a thread on their way at a time (786432 x 128 x 3: 36 us, with four 40)
     if (rl < lanes && hi > lo) {
         const signed char* q = a.q + (p0 + c) * 16;
         for (int64_t row0 = lo + rl; row0 < hi; row0 += U * lanes) {
