@@ -97,9 +97,8 @@ def _quantize(x, dim, pow2):
         scale = _pow2_scale(amax)
         return torch.round(x * (1.0 / scale)), scale
     tiny = amax < 2.0 ** -100                                   # such a row or channel is held as zeros
-    most = torch.full_like(amax, 127.0)                          # a tensor: dividing by a number may multiply by its reciprocal
-    scale = torch.where(tiny, torch.zeros_like(amax), amax / most)
-    inverse = torch.where(tiny, torch.zeros_like(amax), most / amax)
+    scale = torch.where(tiny, torch.zeros_like(amax), amax / 127.0)
+    inverse = torch.where(tiny, torch.zeros_like(amax), 127.0 / amax)
     return torch.round(x * inverse), scale
 
 
