@@ -497,7 +497,7 @@ class GraphedTrainStep:
         if parallel.exchanging():
             raise NotImplementedError("GraphedTrainStep: single process only; use train_step under torch.distributed")
         self.render_fn, self.grad_vars, self.optimizer = render_fn, list(grad_vars), optimizer
-        self.models = list(models)
+        self.models = list({id(m): m for m in models}.values())   # (one network may do both passes)
         if not self.models:
             raise ValueError("GraphedTrainStep: pass the networks the step trains")
         dev = torch.device(device) if device is not None else self.models[0].device
@@ -521,9 +521,9 @@ class GraphedTrainStep:
         held = [m.params for m in self.models]
         leaf = {id(p): p.detach().requires_grad_(True) for ps in held for p in ps}
         self._leaves = [leaf.get(id(v), v) for v in self.grad_vars]
-        for m in self.models:
-            m.params = [leaf[id(p)] for p in m.params]
         try:
+            for m, ps in zip(self.models, held):
+                m.params = [leaf[id(p)] for p in ps]
             self._capture_on_leaves()
         finally:
             for m, ps in zip(self.models, held):

@@ -1,0 +1,44 @@
+"""GraphedTrainStep: what a capture does with the networks it is given."""
+import pytest
+import torch
+
+SHAPE = dict(D=2, W=8, input_ch=3, input_ch_views=3, output_ch=4, skips=[], use_viewdirs=True)
+
+
+def _step(capture, models, grad_vars=None):
+    """A GraphedTrainStep over networks in host memory whose capture is `capture(step)`."""
+    from nerf_amd import training
+
+    class Step(training.GraphedTrainStep):
+        def _capture_on_leaves(self):
+            capture(self)
+    return Step(None, 4, grad_vars if grad_vars is not None else [p for m in models for p in m.params], None, models)
+
+
+def _net():
+    from nerf_amd.run_nerf_helpers import init_nerf_model
+    return init_nerf_model(**SHAPE, device="cpu", precision='int8')
+
+
+@pytest.mark.parametrize("twice", [False, True])
+def test_a_capture_runs_on_leaves_and_leaves_the_parameters_in_place(twice):
+    """... also where one network is listed for both passes, and where the capture fails."""
+    net, other = _net(), _net()
+    models = [net, net] if twice else [net, other]
+    params = [list(m.params) for m in models]
+    seen = []
+
+    def capture(step):
+        for m, ps in zip(models, params):
+            assert all(a is not b and a.data_ptr() == b.data_ptr() and a.is_leaf and a.requires_grad for a, b in zip(m.params, ps))
+        assert [l.data_ptr() for l in step._leaves] == [v.data_ptr() for v in step.grad_vars]
+        assert {id(l) for l in step._leaves} == {id(p) for m in models for p in m.params}
+        seen.append(len(step.models))
+        if len(seen) == 2:
+            raise RuntimeError("no capture")
+    step = _step(capture, models)
+    step._capture()
+    with pytest.raises(RuntimeError, match="no capture"):
+        step._capture()
+    assert seen == [1 if twice else 2] * 2
+    assert all(a is b for m, ps in zip(models, params) for a, b in zip(m.params, ps))
