@@ -517,9 +517,14 @@ class GraphedTrainStep:
         # The networks are captured on leaves of their own over the same memory: a parameter's
         # gradient node lives as long as any graph that holds it and belongs to the stream of that
         # graph, and autograd waits for it at the end of a backward pass, which a capture does not
-        # survive when the stream is another one (the outputs of an eager tape still at hand).
+        # survive when the stream is another one (the outputs of an eager tape still at hand).  Hooks that
+        # a caller registered on the parameters go with them (those of the moment of the capture).
         held = [m.params for m in self.models]
-        leaf = {id(p): p.detach().requires_grad_(True) for ps in held for p in ps}
+        params = {id(p): p for ps in held for p in ps}
+        leaf = {i: p.detach().requires_grad_(True) for i, p in params.items()}
+        for i, p in params.items():
+            for hook in (p._backward_hooks or {}).values():
+                leaf[i].register_hook(hook)
         self._leaves = [leaf.get(id(v), v) for v in self.grad_vars]
         try:
             for m, ps in zip(self.models, held):

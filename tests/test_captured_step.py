@@ -42,3 +42,24 @@ def test_a_capture_runs_on_leaves_and_leaves_the_parameters_in_place(twice):
         step._capture()
     assert seen == [1 if twice else 2] * 2
     assert all(a is b for m, ps in zip(models, params) for a, b in zip(m.params, ps))
+
+
+def test_hooks_of_parameters_take_part_in_a_capture():
+    """A hook on a parameter changes the gradient that tape.gradient returns; it does so on the capture's leaves too,
+    in the order of registration, and a removed one does not."""
+    net = _net()
+    calls, out = [], []
+    net.params[0].register_hook(lambda g: g * 3)
+    net.params[0].register_hook(lambda g: g + 1)
+    net.params[2].register_hook(lambda g: calls.append(float(g.sum())))
+    net.params[4].register_hook(lambda g: g * 0).remove()
+
+    def capture(step):
+        from nerf_amd import training
+        with training.GradientTape() as tape:
+            loss = sum((p * (i + 1)).sum() for i, p in enumerate(net.params))
+        out.append(tape.gradient(loss, step._leaves))
+    _step(capture, [net])._capture()
+    want = [torch.full_like(p, i + 1.) for i, p in enumerate(net.params)]
+    want[0] = want[0] * 3 + 1
+    assert all(torch.equal(a, b) for a, b in zip(out[0], want)) and calls == [3. * net.params[2].numel()]
