@@ -193,6 +193,8 @@ class NerfModel:
 
     def packed_bwd(self):
         """The transposed stream the gradient chain reads."""
+        if self.layered:
+            raise NotImplementedError("a layered network has no fused weight stream")
         ver = self._version()
         if self._packed_bwd is None:
             self._packed_bwd = torch.empty((ops.packed_bwd_bytes(),), dtype=torch.uint8, device=self.device)
