@@ -16,7 +16,7 @@ import torch
 
 from . import _native as nv
 from . import ops
-from .run_nerf_helpers import NerfModel
+from .run_nerf_helpers import LaidOut, NerfModel
 
 _QUERY_POINTS = 1 << 20   # points evaluated at a time when nothing is recorded: bounds the transient memory
 
@@ -28,8 +28,7 @@ class LayeredNerfModel(NerfModel):
 
     def __init__(self, D, W, input_ch, input_ch_views, output_ch, skips, use_viewdirs, device=None, generator=None):
         super().__init__(D, W, input_ch, input_ch_views, output_ch, skips, use_viewdirs, device=device, generator=generator)
-        self._packed8 = None
-        self._packed8_version = None
+        self._packed8 = LaidOut(self.device)
 
     @staticmethod
     def check_shape(D, W, input_ch, input_ch_views, output_ch, skips, use_viewdirs):
@@ -65,14 +64,11 @@ class LayeredNerfModel(NerfModel):
     def packed8(self):
         """Per layer its Int8Weights, one for each part of split(), for the current parameters (re-laid in the
         same memory when they change, also by a captured graph)."""
-        ver = self._version()
-        if ver != self._packed8_version:
-            old = self._packed8
-            with torch.no_grad():
-                self._packed8 = [[ops.pack_int8(self.weight(i)[r0:r0 + n], pow2=True, into=old[i][j] if old else None)
-                                  for j, (r0, n, _) in enumerate(self.split(i))] for i in range(len(self.shapes))]
-            self._packed8_version = ver
-        return self._packed8
+
+        def lay(old):
+            return [[ops.pack_int8(self.weight(i)[r0:r0 + n], pow2=True, into=old[i][j] if old else None)
+                     for j, (r0, n, _) in enumerate(self.split(i))] for i in range(len(self.shapes))]
+        return self._packed8.current(self._version(), lay, lambda layers: (w.packed for parts in layers for w in parts))
 
 
 def _encode(x, channels):
@@ -86,7 +82,7 @@ class _Pass:
         """pts [P, 3], viewdirs [P / S, 3], all fp32."""
         self.model = model
         packed = model.packed8()
-        self.version = model._packed8_version
+        self.version = model._version()
         D = model.D
         pe = ops.quantize_rows(_encode(pts, model.input_ch), pow2=True)
         # one encoding per ray, its integers repeated for the ray's points
@@ -118,9 +114,10 @@ class _Pass:
 
     def gradients(self, d_raw):
         """Gradients of the parameters, in their order, from d raw [P, 4] fp32."""
-        model, packed, D = self.model, self.model.packed8(), self.model.D
-        if model._packed8_version != self.version:
+        model, D = self.model, self.model.D
+        if model._version() != self.version:
             raise RuntimeError("the network's parameters changed between its forward and its backward pass")
+        packed = model.packed8()
         grads = [None] * len(model.params)
 
         def parameters(i, dz):

@@ -77,6 +77,46 @@ def get_embedder(multires, i=0):
 _MODELS_BY_STORAGE = weakref.WeakValueDictionary()
 
 
+class LaidOut:
+    """One layout of a network's weights for the kernels, kept from call to call and written anew, in the same
+    memory, when the parameters change.  Every stream may use it: the one that finds the parameters changed queues the
+    layout, a call on another waits on the device until it is there.  (That a change of the parameters waits for the
+    calls that still read them is the caller's part: those calls read the biases themselves.)"""
+
+    def __init__(self, device):
+        self.device, self.memory, self.version = device, None, None
+        self.stream = self.event = None   # where the last layout was queued, and the point behind it
+        self.known = set()                # streams the allocator knows to use the memory
+
+    def __reduce__(self):                 # a copy of a network lays out its own
+        return LaidOut, (self.device,)
+
+    def current(self, version, lay, tensors=lambda memory: (memory,)):
+        """The memory, laid out for the parameters of that version; lay(memory, or None the first time) queues a
+        layout on the current stream and returns the memory.  tensors(memory): the tensors it consists of."""
+        if self.device.type != 'cuda':
+            self.memory, self.version = lay(self.memory), version
+            return self.memory
+        stream = torch._C._cuda_getCurrentRawStream(self.device.index)
+        if version == self.version and stream == self.stream:
+            return self.memory
+        with torch.no_grad(), torch.cuda.device(self.device):
+            capturing = torch.cuda.is_current_stream_capturing()   # (a capture begins with the device idle)
+            here = torch.cuda.current_stream()
+            if not capturing and self.event is not None and stream != self.stream:
+                here.wait_event(self.event)
+            if version != self.version:
+                self.memory, self.version = lay(self.memory), version
+                if not capturing:
+                    self.stream, self.event = stream, torch.cuda.Event()
+                    self.event.record(here)
+            if not capturing and stream not in self.known:
+                self.known.add(stream)
+                for t in tensors(self.memory):
+                    t.record_stream(here)
+        return self.memory
+
+
 class NerfModel:
     """What init_nerf_model returns: the parameters of one network with the slice of the Keras
     Model interface create_nerf and train() use (get_weights / set_weights / trainable_variables,
@@ -129,10 +169,8 @@ class NerfModel:
             at += fo
             self.params.append(w.requires_grad_(True))
             self.params.append(bvec.requires_grad_(True))
-        self._packed = torch.empty((ops.packed_bytes(),), dtype=torch.uint8, device=dev) if dev.type == 'cuda' and not self.layered else None
-        self._packed_bwd = None
-        self._packed_version = None
-        self._packed_bwd_version = None
+        self._packed = LaidOut(dev)
+        self._packed_bwd = LaidOut(dev)
         self._epoch = 0          # bumped by updates that bypass torch (the fused Adam kernel)
         # factor applied to d_raw before the fp16 gradient chain; None = formed on the device from
         # max|d_raw| at every backward pass (what callers should leave it at) so that the largest
@@ -184,25 +222,25 @@ class NerfModel:
         """The fp16 fragment stream for the current parameter values (re-packed when they change)."""
         if self.layered:
             raise NotImplementedError("a layered network has no fused weight stream")
-        ver = self._version()
-        if ver != self._packed_version:
-            with torch.no_grad():
-                ops.mlp_pack([p.detach() for p in self.params], self._packed)
-            self._packed_version = ver
-        return self._packed
+
+        def lay(memory):
+            if memory is None:
+                memory = torch.empty((ops.packed_bytes(),), dtype=torch.uint8, device=self.device)
+            ops.mlp_pack([p.detach() for p in self.params], memory)
+            return memory
+        return self._packed.current(self._version(), lay)
 
     def packed_bwd(self):
         """The transposed stream the gradient chain reads."""
         if self.layered:
             raise NotImplementedError("a layered network has no fused weight stream")
-        ver = self._version()
-        if self._packed_bwd is None:
-            self._packed_bwd = torch.empty((ops.packed_bwd_bytes(),), dtype=torch.uint8, device=self.device)
-        if ver != self._packed_bwd_version:
-            with torch.no_grad():
-                ops.mlp_pack_bwd([p.detach() for p in self.params], self._packed_bwd)
-            self._packed_bwd_version = ver
-        return self._packed_bwd
+
+        def lay(memory):
+            if memory is None:
+                memory = torch.empty((ops.packed_bwd_bytes(),), dtype=torch.uint8, device=self.device)
+            ops.mlp_pack_bwd([p.detach() for p in self.params], memory)
+            return memory
+        return self._packed_bwd.current(self._version(), lay)
 
     def grad_status(self):
         """(flags, gscale_used, max|d_raw|) of this network's last backward pass; flags is a
