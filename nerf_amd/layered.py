@@ -81,7 +81,7 @@ class _Pass:
     def __init__(self, model, pts, viewdirs, S):
         """pts [P, 3], viewdirs [P / S, 3], all fp32."""
         self.model = model
-        packed = model.packed8()
+        packed = self.packed = model.packed8()
         self.version = model._version()
         D = model.D
         pe = ops.quantize_rows(_encode(pts, model.input_ch), pow2=True)
@@ -114,10 +114,9 @@ class _Pass:
 
     def gradients(self, d_raw):
         """Gradients of the parameters, in their order, from d raw [P, 4] fp32."""
-        model, D = self.model, self.model.D
+        model, packed, D = self.model, self.packed, self.model.D
         if model._version() != self.version:
             raise RuntimeError("the network's parameters changed between its forward and its backward pass")
-        packed = model.packed8()
         grads = [None] * len(model.params)
 
         def parameters(i, dz):

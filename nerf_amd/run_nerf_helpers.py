@@ -81,7 +81,10 @@ class LaidOut:
     """One layout of a network's weights for the kernels, kept from call to call and written anew, in the same
     memory, when the parameters change.  Every stream may use it: the one that finds the parameters changed queues the
     layout, a call on another waits on the device until it is there.  (That a change of the parameters waits for the
-    calls that still read them is the caller's part: those calls read the biases themselves.)"""
+    calls that still read them is the caller's part: those calls read the biases themselves.)  In a graph capture a
+    layout of changed parameters is part of the graph, made at every replay and not before, so that calls outside do not
+    count on it; a layout that is current is read as it is: a graph that shall follow the parameters is captured
+    after mark_dirty()."""
 
     def __init__(self, device):
         self.device, self.memory, self.version = device, None, None
@@ -106,9 +109,9 @@ class LaidOut:
             if not capturing and self.event is not None and stream != self.stream:
                 here.wait_event(self.event)
             if version != self.version:
-                self.memory, self.version = lay(self.memory), version
+                self.memory = lay(self.memory)
                 if not capturing:
-                    self.stream, self.event = stream, torch.cuda.Event()
+                    self.version, self.stream, self.event = version, stream, torch.cuda.Event()
                     self.event.record(here)
             if not capturing and stream not in self.known:
                 self.known.add(stream)

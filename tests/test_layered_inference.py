@@ -70,3 +70,26 @@ def test_a_copied_network_lays_out_its_own_weights(gpu, precision):
     twin = copy.deepcopy(net)
     twin.set_weights(other.get_weights())
     assert torch.equal(query(twin, rays, z), want) and torch.equal(query(net, rays, z), held)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("precision", ['int8', None])
+def test_weights_laid_out_in_a_capture_are_not_there_yet(gpu, precision):
+    """A query captured when the parameters have just changed lays them out at every replay; until the first one, calls
+    outside of the graph do it themselves.  Every replay follows the parameters."""
+    (net, other), query = _networks(gpu, precision)
+    rays, z = _rays(gpu, 30, 5)
+    old, want = query(net, rays, z), query(other, rays, z)
+    weights = [[w.copy() for w in m.get_weights()] for m in (net, other)]
+    net.set_weights(weights[1])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = query(net, rays, z)
+    assert torch.equal(query(net, rays, z), want)           # eager, before any replay
+    for turn in range(4):
+        net.set_weights(weights[turn % 2])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want if turn % 2 else old)
+        assert torch.equal(query(net, rays, z), want if turn % 2 else old)
