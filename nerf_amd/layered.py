@@ -1,10 +1,12 @@
 """The reference's network (run_nerf_helpers.py:80-117) evaluated and trained layer by layer on the 8-bit
 dense-layer kernels, for the widths and depths the fused kernels are not built for.
 
-Every layer's input is held in 8-bit integers with one scale per point; a hidden layer is one launch that
-reads the integers of the layer before and leaves its own (ops.linear_int8_quantized), so a point's
-activations never exist in more than 8 bits, and the integers, scales and ReLU bits are all that the
-backward pass keeps: about 2.8 KB per point of the 8 x 256 network, where the fused kernels save 4.7 KB.
+Every layer's input is held in 8-bit integers with one scale per point; a hidden layer reads the integers of the
+layer before and leaves its own (ops.linear_int8_quantized: one launch, but for layers wider than 512 and for few
+points, where it may be two with an fp32 row in between).  The layers that take an encoding beside the layer before
+have one product for each, the encoding's being added in the epilogue of the other.  For the backward pass the
+integers, scales and ReLU bits are all that is kept: about 2.8 KB per point of the 8 x 256 network, where the fused
+kernels save 4.7 KB.  A query that records nothing keeps one layer at a time and makes no bits.
 Gradients between layers are bf16, parameter gradients fp32; rounding to 8 bits passes gradients on
 unchanged.
 
@@ -18,7 +20,10 @@ from . import _native as nv
 from . import ops
 from .run_nerf_helpers import LaidOut, NerfModel
 
-_QUERY_POINTS = 1 << 20   # points evaluated at a time when nothing is recorded: bounds the transient memory
+# Points evaluated at a time when nothing is recorded: no more than these, and as many as the network's widest layer
+# leaves within these bytes of transient memory (one 256 wide takes 2.3 GiB for its 2^20, one 4096 wide 89 thousand points).
+_QUERY_POINTS = 1 << 20
+_QUERY_BYTES = 4 << 30
 
 
 class LayeredNerfModel(NerfModel):
@@ -71,15 +76,42 @@ class LayeredNerfModel(NerfModel):
         return self._packed8.current(self._version(), lay, lambda layers: (w.packed for parts in layers for w in parts))
 
 
+def _row_bytes(k):
+    return -(-k // 64) * 64 + 4
+
+
+def point_bytes(model):
+    """Upper bound of the device memory that a point takes in a pass that records nothing: both encodings (fp32 and 8 bits),
+    and of one layer its input rows, its output rows, an addend and an fp32 row (where ops.linear_int8_quantized makes two
+    calls), and the four outputs twice."""
+    both = model.input_ch, model.input_ch_views
+    layer = max(sum(_row_bytes(n) for _, n, _ in model.split(i)) + _row_bytes(m) + 8 * m for i, (_, m) in enumerate(model.shapes))
+    return sum(_row_bytes(c) + 4 * c for c in both) + layer + 2 * 16
+
+
+def query_points(model):
+    return max(1, min(_QUERY_POINTS, _QUERY_BYTES // point_bytes(model)))
+
+
+def _pieces(P, S, most):
+    """(first point, one behind the last, first ray, points per ray) of pieces of at most `most` points: whole rays, or parts
+    of one where a ray's S points are more than that."""
+    if S <= most:
+        step = most // S * S
+        return [(a, min(a + step, P), a // S, S) for a in range(0, P, step)]
+    return [(a, min(a + most, r * S + S), r, min(most, r * S + S - a)) for r in range(P // S) for a in range(r * S, r * S + S, most)]
+
+
 def _encode(x, channels):
     return ops.embed(x, (channels - 3) // 6) if channels > 3 else x
 
 
 class _Pass:
-    """One forward pass: rows of every layer's input, in the order of split()."""
+    """One forward pass: raw [P, 4], and for gradients() the rows of every layer's input, in the order of split()."""
 
-    def __init__(self, model, pts, viewdirs, S):
-        """pts [P, 3], viewdirs [P / S, 3], all fp32."""
+    def __init__(self, model, pts, viewdirs, S, record=True):
+        """pts [P, 3], viewdirs [P / S, 3], all fp32.  record: whether rows and ReLU bits are kept (without, a layer's rows
+        go when the next layer's are there, and no bits are made)."""
         self.model = model
         packed = self.packed = model.packed8()
         self.version = model._version()
@@ -92,7 +124,8 @@ class _Pass:
 
         def dense(i, parts, **out):
             # the narrow part of a concatenated input first, as the addend of the other
-            self.inputs[i] = parts
+            if record:
+                self.inputs[i] = parts
             add = None
             at = [j for j, (_, _, enc) in enumerate(model.split(i)) if not enc or len(parts) == 1][0]
             for j, rows in enumerate(parts):
@@ -104,12 +137,12 @@ class _Pass:
 
         h = [pe]
         for i in range(D):
-            y = dense(i, h, relu=True, want_mask=True)
+            y = dense(i, h, relu=True, want_mask=record)
             h = [pe, y] if i in model.skips else [y]
         alpha = dense(D + 3, h, dtype=torch.float32)
-        bott = dense(D, h)
-        v = dense(D + 1, [bott, ve], relu=True, want_mask=True)
-        rgb = dense(D + 2, [v], dtype=torch.float32)
+        h = [dense(D, h), ve]
+        h = [dense(D + 1, h, relu=True, want_mask=record)]
+        rgb = dense(D + 2, h, dtype=torch.float32)
         self.raw = torch.cat([rgb, alpha], dim=1)
 
     def gradients(self, d_raw):
@@ -153,10 +186,14 @@ def query(model, pts, viewdirs, S):
     P = pts.shape[0]
     if P == 0:
         return pts.new_empty((0, 4))
-    step = max(_QUERY_POINTS // S, 1)
+    pieces = _pieces(P, S, query_points(model))
     with torch.no_grad():
-        out = [_Pass(model, pts[i * S:(i + step) * S], viewdirs[i:i + step], S).raw for i in range(0, P // S, step)]
-    return out[0] if len(out) == 1 else torch.cat(out, 0)
+        if len(pieces) == 1:
+            return _Pass(model, pts, viewdirs, S, record=False).raw
+        out = pts.new_empty((P, 4))
+        for a, b, ray, s in pieces:
+            out[a:b] = _Pass(model, pts[a:b], viewdirs[ray:ray + (b - a) // s], s, record=False).raw
+        return out
 
 
 class LayeredQuery(torch.autograd.Function):

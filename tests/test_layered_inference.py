@@ -15,6 +15,68 @@ def test_the_fused_streams_of_a_layered_network_are_refused():
                 call()
 
 
+# ---- memory of a query ----------------------------------------------------------------------------------
+@pytest.mark.parametrize("P,S,most", [(0, 5, 7), (12, 4, 100), (12, 4, 12), (12, 4, 11), (12, 4, 4), (12, 4, 3), (12, 4, 1), (1000, 1, 64), (777, 777, 100), (2100, 700, 333)])
+def test_pieces_of_a_query(P, S, most):
+    """Every point once and in order, with its ray, and no piece larger than asked for."""
+    from nerf_amd.layered import _pieces
+    at = 0
+    for a, b, ray, s in _pieces(P, S, most):
+        assert a == at and 0 < b - a <= most and (b - a) % s == 0
+        assert all((p - a) // s + ray == p // S for p in range(a, b))
+        at = b
+    assert at == P
+
+
+@pytest.mark.parametrize("change,points", [(dict(D=8, W=256, input_ch=63, input_ch_views=27, skips=[4]), 1 << 20), (dict(D=2, W=2, skips=[]), 1 << 20),
+                                           (dict(D=64, W=4096, skips=[]), None), (dict(D=1, W=4096, input_ch=63, skips=[0]), None)])
+def test_the_points_of_a_query_go_by_the_widest_layer(change, points, monkeypatch):
+    from nerf_amd import layered
+    # (without the parameters, which a 64 x 4096 network has 4 GiB of)
+    net = type('Net', (), dict(split=layered.LayeredNerfModel.split))()
+    s = {**SHAPE, **change}
+    net.D, net.W, net.input_ch, net.input_ch_views, net.skips = s['D'], s['W'], s['input_ch'], s['input_ch_views'], s['skips']
+    k, net.shapes = net.input_ch, []
+    for i in range(net.D):
+        net.shapes.append((k, net.W))
+        k = net.W + (net.input_ch if i in net.skips else 0)
+    net.shapes += [(k, 256), (256 + net.input_ch_views, net.W // 2), (net.W // 2, 3), (k, 1)]
+    got = layered.query_points(net)
+    assert points is None or got == points
+    # two rows of integers and an fp32 row of the widest layer are below the bound, and the budget above it
+    assert layered.point_bytes(net) >= 2 * net.W + 4 * net.W and got * layered.point_bytes(net) <= layered._QUERY_BYTES
+    monkeypatch.setattr(layered, '_QUERY_BYTES', 1)
+    assert layered.query_points(net) == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("change", [dict(D=12, W=700, skips=[3]), dict(D=5, W=256, input_ch=63, input_ch_views=27, skips=[0, 2]), dict(D=3, W=1100, skips=[])])
+def test_a_query_stays_within_its_memory(gpu, change, monkeypatch):
+    """The peak of a query, beside its result and a piece of fragments, is within the bytes that it is given, whatever the
+    depth; its result is that of one piece, and of a pass that records."""
+    from nerf_amd import layered
+    from nerf_amd.run_nerf_helpers import init_nerf_model
+    net = init_nerf_model(**{**SHAPE, **change}, device=gpu, generator=torch.Generator(device=gpu).manual_seed(7), precision='int8')
+    n, S = 4000, 9
+    pts = torch.rand((n * S, 3), device=gpu) * 2 - 1
+    vd = torch.nn.functional.normalize(torch.randn((n, 3), device=gpu), dim=1)
+    want = layered._Pass(net, pts, vd, S).raw
+    assert torch.equal(layered.query(net, pts, vd, S), want)
+    budget = 16 << 20
+    monkeypatch.setattr(layered, '_QUERY_BYTES', budget)
+    assert layered.query_points(net) < n * S / 3
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = layered.query(net, pts, vd, S)
+    peak = torch.cuda.max_memory_allocated() - before - got.numel() * 4
+    assert torch.equal(got, want)
+    assert peak <= budget + (1 << 20), (peak, layered.query_points(net), layered.point_bytes(net))   # (blocks are rounded to 512 bytes)
+    monkeypatch.setattr(layered, '_QUERY_BYTES', 4 * layered.point_bytes(net))                       # parts of one ray
+    assert torch.equal(layered.query(net, pts[:5 * S], vd[:5], S), want[:5 * S])
+
+
 # ---- streams ---------------------------------------------------------------------------------------
 def _rays(gpu, n, seed):
     g = torch.Generator(device=gpu).manual_seed(seed)
