@@ -123,14 +123,15 @@ class _Pass:
         self.inputs = [None] * len(model.shapes)
 
         def dense(i, parts, **out):
-            # the narrow part of a concatenated input first, as the addend of the other
+            # the narrow part of a concatenated input first, as the addend of the other: a partial sum, in fp32 (in bf16 it
+            # would save 5 % of a training step and 14 % of a query)
             if record:
                 self.inputs[i] = parts
             add = None
             at = [j for j, (_, _, enc) in enumerate(model.split(i)) if not enc or len(parts) == 1][0]
             for j, rows in enumerate(parts):
                 if j != at:
-                    add = ops.linear_int8(rows, packed[i][j], dtype=torch.bfloat16)
+                    add = ops.linear_int8(rows, packed[i][j])
             if 'dtype' in out:
                 return ops.linear_int8(parts[at], packed[i][at], model.bias(i), addend=add, **out)
             return ops.linear_int8_quantized(parts[at], packed[i][at], model.bias(i), addend=add, pow2=True, **out)

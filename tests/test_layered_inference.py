@@ -155,3 +155,26 @@ def test_weights_laid_out_in_a_capture_are_not_there_yet(gpu, precision):
         torch.cuda.synchronize()
         assert torch.equal(out, want if turn % 2 else old)
         assert torch.equal(query(net, rays, z), want if turn % 2 else old)
+
+
+# ---- accuracy -------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("W", [40, 256, 600])
+def test_a_concatenated_layer_adds_its_parts_in_32_bits(gpu, W):
+    """The density head behind a skip has the encoding and a layer as inputs and leaves fp32: against 64 bits, from the
+    integers it read.  Each part: the sum and two scales, three roundings of 2^-24 of it; bias and addend one more each."""
+    from nerf_amd.layered import _Pass
+    from nerf_amd.run_nerf_helpers import init_nerf_model
+    from tests.test_int8_layers import close, dequantised, ref_linear
+    net = init_nerf_model(**{**SHAPE, 'D': 2, 'W': W, 'skips': [1]}, device=gpu, generator=torch.Generator(device=gpu).manual_seed(1), precision='int8')
+    pts = torch.rand((500, 3), device=gpu) * 2 - 1
+    run = _Pass(net, pts, torch.nn.functional.normalize(torch.randn((100, 3), device=gpu), dim=1), 5)
+    head = net.D + 3
+    assert [enc for _, _, enc in net.split(head)] == [True, False]
+    want = net.bias(head).detach().double()
+    mag = want.abs()
+    for rows, (r0, k, _) in zip(run.inputs[head], net.split(head)):
+        p, s, _ = ref_linear(rows, net.weight(head)[r0:r0 + k].detach(), True)
+        want = want + dequantised(rows) @ (p * s)
+        mag = mag + (dequantised(rows) @ (p * s)).abs()
+    close(run.raw[:, 3:], want, 5.001 * 2.0 ** -24 * mag, "alpha")
