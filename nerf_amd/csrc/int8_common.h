@@ -204,20 +204,27 @@ DEV unsigned low_bytes(const float (&t)[4]) {
 // How many bf16 numbers a value of a type is the exact sum of (8, 11 and 24 bits of 8 each).
 template <int DT> struct Terms { static constexpr int N = DT == NERF_BF16 ? 1 : DT == NERF_F16 ? 2 : 3; };
 
-// v as the sum of N bf16 terms, each the rounding of what the ones before it leave.  (An infinite v, or one
-// within half a bf16 step of the fp32 maximum, leaves NaN in the second term, so its sums are NaN.)
+// v as the sum of N bf16 terms, each the leading bits (cut off, not rounded: a value near the fp32 maximum would
+// round to infinity) of what the ones before it leave: exact down to bf16's smallest steps.  An infinity is its
+// first term, with zeros behind; a NaN is one in the first or the second.
 template <int N>
 DEV void split_bf16(const float (&v)[8], bf16x8 (&t)[N]) {
-    float rest[8];
+    unsigned rest[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) rest[i] = v[i];
+    for (int i = 0; i < 8; ++i) rest[i] = __builtin_bit_cast(unsigned, v[i]);
 #pragma unroll
     for (int s = 0; s < N; ++s) {
+        i32x4 w;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const __bf16 b = (__bf16)rest[i];
-            t[s][i] = b;
-            if (s + 1 < N) rest[i] -= (float)b;
+        for (int i = 0; i < 4; ++i) w[i] = (int)__builtin_amdgcn_perm(rest[2 * i + 1], rest[2 * i], 0x07060302u);
+        t[s] = __builtin_bit_cast(bf16x8, w);
+        if (s + 1 < N) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float left = __builtin_bit_cast(float, rest[i]) - __builtin_bit_cast(float, rest[i] & 0xffff0000u);
+                const bool inf = s == 0 && __builtin_fabsf(v[i]) == __builtin_inff();
+                rest[i] = inf ? 0u : __builtin_bit_cast(unsigned, left);
+            }
         }
     }
 }
