@@ -195,13 +195,9 @@ DEV void store_piece(T* dst, int have, bool whole, const float* v) {
     }
 }
 
-// A NaN with its sign bit clear, which the integer form of relu keeps; anything else as it is.
-DEV float positive_nan(float v) { return v != v ? __builtin_bit_cast(float, 0x7fc00000u) : v; }
-
 // y = relu((sum x channel scale) x row scale + bias + addend): the sum rounded to fp32, its product with
 // the channel scale rounded, then one rounding for row scale and bias and one for the addend.  ws, b: the
-// channels' scales and biases of the group of 64 from f0 (0 and 0 behind the last channel; a NaN without
-// its sign).
+// channels' scales and biases of the group of 64 from f0 (0 and 0 behind the last channel).
 template <int OUT, int ADD>
 DEV void finish_linear(const LinearArgs& a, const i32x4 (&acc)[4], const float* ws, const float* b, float xs, int f0, int g,
                        int64_t p, bool whole, bool relu, float (&v)[16]) {
@@ -220,15 +216,10 @@ DEV void finish_linear(const LinearArgs& a, const i32x4 (&acc)[4], const float* 
             const int f = f0 + feature_of<OUT>(i, g);
             add_piece<A, kPiece<OUT>>(row + f, a.features - f, whole, v + i);
         }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = positive_nan(v[i]);
     }
-    if (relu) {  // a negative float is a negative integer: one instruction, and a NaN stays one
+    if (relu) {  // (v_maximum3_f32: a NaN of either sign stays one)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int bits = __builtin_bit_cast(int, v[i]);
-            v[i] = __builtin_bit_cast(float, bits > 0 ? bits : 0);
-        }
+        for (int i = 0; i < 16; ++i) v[i] = __builtin_elementwise_maximum(v[i], 0.f);
     }
 }
 
@@ -299,7 +290,7 @@ DEV void stage_channels(const LinearArgs& a, float* ws, float* b, int f0, int co
     for (int i = threadIdx.x; i < count; i += blockDim.x) {
         const int f = f0 + i;
         ws[i] = f < a.features ? a.wscale[f] : 0.f;
-        b[i] = (a.bias && f < a.features) ? positive_nan(a.bias[f]) : 0.f;
+        b[i] = (a.bias && f < a.features) ? a.bias[f] : 0.f;
     }
 }
 
@@ -349,7 +340,7 @@ __global__ __launch_bounds__(256) void linear_direct_kernel(LinearArgs a) {
         // this wave's 64 channels, through its own piece of LDS (one wave: in order, no barrier)
         const int c = 64 * T + lane;
         ch[wave][0][lane] = c < a.features ? a.wscale[c] : 0.f;
-        ch[wave][1][lane] = (a.bias && c < a.features) ? positive_nan(a.bias[c]) : 0.f;
+        ch[wave][1][lane] = (a.bias && c < a.features) ? a.bias[c] : 0.f;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
 #pragma unroll

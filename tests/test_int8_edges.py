@@ -78,3 +78,38 @@ def test_gradients_of_the_largest_and_smallest_size(gpu, n, k, m):
         close(ops.linear_int8_grad_input(d32, packed), want, mag * (3 * m * 2.0 ** -23 + 2.0 ** -24) + lost * wd.abs().sum(1) + 1e-38, name + " dx")
         dw, _ = ops.linear_int8_grad_weight(rows, d32)
         close(dw, xd.t().contiguous() @ d, xd.abs().t().contiguous() @ d.abs() * 3 * n * 2.0 ** -23 + lost * xd.abs().sum(0)[:, None] + 1e-38, name + " dW")
+
+
+@gpu_only
+@pytest.mark.parametrize("n,k,m", [(40, 70, 96), (33000, 256, 192), (16500, 700, 704), (16500, 512, 512), (9000, 256, 576)])
+def test_a_nan_of_either_sign_passes_a_relu(gpu, n, k, m):
+    """A row's scale, a bias, an addend that is NaN with its sign bit set, and the difference of two infinities."""
+    from nerf_amd import ops
+    x, w, _, b = make(n, k, m, 7, gpu)
+    rows, packed = ops.quantize_rows(x.abs() + 0.1), ops.pack_int8(w)
+    neg = torch.tensor([-1], dtype=torch.int32, device=gpu).view(torch.float32)
+    at = [0, n // 2, n - 1]
+
+    def check(y, q, where, col=slice(None)):
+        assert bool(torch.isnan(y[where, col]).all())
+        assert bool(torch.isnan(q.scale[where]).all()) and not bool(q.q[where].any())
+    scale = rows.scale.clone()
+    scale[at] = neg
+    bad = ops.Int8Rows(rows.q, scale, k)
+    bias = b.clone()
+    bias[m // 2] = neg[0]
+    add = torch.zeros((n, m), device=gpu)
+    add[at] = neg
+    both = lambda *a, **kw: (ops.linear_int8(*a, relu=True, **kw), ops.linear_int8_quantized(*a, relu=True, want_mask=True, **kw))
+    check(*both(bad, packed, b), at)
+    check(*both(rows, packed, bias), slice(None), m // 2)
+    check(*both(rows, packed, b, addend=add), at)
+    # sums of either sign times an infinite scale, plus the other infinity
+    inf = float("inf")
+    scale[at] = inf
+    sums = ops.linear_int8(ops.Int8Rows(rows.q, torch.ones_like(scale), k), packed)[0]
+    opposite = torch.where(sums > 0, torch.full_like(b, -inf), torch.full_like(b, inf))
+    y, q = both(ops.Int8Rows(rows.q, scale, k), packed, opposite)
+    check(y[:1], q, slice(0, 1))
+    want = torch.relu(opposite)
+    assert torch.equal(y[1], want)                           # a finite row plus an infinite bias
