@@ -596,18 +596,30 @@ def linear_int8(rows, weights, bias=None, relu=False, addend=None, dtype=torch.f
     return y
 
 
+def _through_fp32(n, k, m):
+    """Whether an 8-bit output of these sizes is faster by way of a stored fp32 row, in two calls.  Device time, one call / two
+    calls, us:
+     - up to 512 outputs a row is one workgroup's, which walks its inputs step by step: with few rows of many inputs the
+       many small workgroups of the product alone are faster, weights in LDS or not.  640 x 64, 2048 rows 10.7 / 9.6, 12288
+       rows 11.0 / 11.1; 896 x 128, 8192 rows 14.3 / 13.2; 640 x 256, 8192 rows 17.8 / 14.6, 12288 rows 17.9 / 21.4; 640 x 512,
+       4096 rows 18.3 / 15.2, 8192 rows 18.8 / 26.7.  Up to 576 inputs the two are close, and one call is less host time;
+     - beyond, the products are formed twice.  With few tiles: 256 x 576, 4096 rows 21.2 / 16.1, 8192 rows 21.9 / 25.2; 512 x
+       2048, 2048 rows 29.0 / 23.5, 4096 rows 30.1 / 35.0.  With many inputs: 640 x 1024, 32768 rows 66 / 69, 896 x 1024 79 /
+       77, 1024 x 1024 87 / 79; once the fp32 rows do not stay in the 256 MB cache in front of memory: 1024 x 1024, 131072
+       rows 317 / 369, 1280 x 1024 369 / 401, 2048 x 2048, 32768 rows 271 / 240."""
+    groups = -(-m // 64)
+    if m <= 512:
+        return k > 576 and n < 12288 and n * groups < 40960
+    return n * groups <= 65536 or k > (768 if n * m * 4 <= 256 << 20 else 1280)
+
+
 def linear_int8_quantized(rows, weights, bias=None, relu=False, addend=None, pow2=False, want_mask=False):
     """quantize_rows(linear_int8(...), pow2, want_mask), with y in fp32 in between: the next layer's input.  One
     call that never stores y, but where storing it is faster or an addend is not a multiple of 64 wide: the two
     calls."""
     dev, bias, addend, add_dtype, ldadd = _linear_inputs("linear_int8_quantized", rows, weights, bias, addend)
-    # (one call, two calls, us.  Up to 512 outputs a row forms in one workgroup: with few rows of over 576 inputs,
-    # whose weights are not resident, few of those run and each waits for one step of inputs after the other.  1024 x 256,
-    # 8192 rows 21, 15, 16384 rows 21, 35; 512 x 512, 4096 rows 15, 14, 16384 rows 16, 31.  Beyond, the products are formed
-    # twice.  500 x 1000, 300 rows 32, 17; 256 x 1024, 8192 rows 22, 29; 32768 rows, 512 x 1024 65, 73, 1024 x 1024 89,
-    # 85, 2048 x 1024 136, 108; 120 x 1271, 162501 rows 218, 437)
     n, m = rows.n, weights.m
-    if (addend is not None and m % 64 != 0) or (rows.k > 576 and n < 12288) or (m > 512 and (n < 4096 or rows.k > 1024)):
+    if (addend is not None and m % 64 != 0) or _through_fp32(n, rows.k, m):
         return quantize_rows(linear_int8(rows, weights, bias, relu, addend), pow2, want_mask)
     q, scale, mask = _new_rows(n, m, dev, want_mask)
     need = nv.lib().nerf_linear_int8_quantized_bytes(n, m) if m > 512 else 0

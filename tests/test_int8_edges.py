@@ -113,3 +113,12 @@ def test_a_nan_of_either_sign_passes_a_relu(gpu, n, k, m):
     check(y[:1], q, slice(0, 1))
     want = torch.relu(opposite)
     assert torch.equal(y[1], want)                           # a finite row plus an infinite bias
+
+
+@pytest.mark.parametrize("n,k,m,two", [(2048, 640, 64, True), (16384, 640, 64, False), (8192, 896, 128, True), (8192, 640, 256, True), (12288, 640, 256, False),
+                                       (4096, 640, 512, True), (8192, 640, 512, False), (100, 576, 256, False), (1, 64, 512, False),
+                                       (4096, 256, 576, True), (8192, 256, 576, False), (2048, 512, 2048, True), (4096, 512, 2048, False),
+                                       (32768, 640, 1024, False), (32768, 1024, 1024, True), (131072, 1024, 1024, False), (32768, 2048, 2048, True), (162501, 120, 1271, False)])
+def test_an_8_bit_output_takes_the_way_that_was_measured_faster(n, k, m, two):
+    from nerf_amd import ops
+    assert ops._through_fp32(n, k, m) is two
