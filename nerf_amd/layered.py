@@ -10,6 +10,12 @@ kernels save 4.7 KB.  A query that records nothing keeps one layer at a time and
 Gradients between layers are bf16, parameter gradients fp32; rounding to 8 bits passes gradients on
 unchanged.
 
+The encoded point is one row, coordinates and sines under one scale, the next power of two of its largest value over
+127: the sines' step is 1/64 while every coordinate is below 1.98 in size, 1/32 below 3.97, 1/16 below 7.9.  Scenes are
+best scaled to about +-2.  Off the same network in 64 bits (8 x 256, rms, in standard deviations of the density and
+colour outputs): 3.5 and 1.8 % with coordinates up to 2, 3.7 and 2.1 % up to 4, 4.1 and 2.3 % up to 6 (with coordinates and
+sines apart 3.3 and 2.1 % there: most of it is the layers' own rounding).
+
     model = init_nerf_model(D=4, W=128, input_ch=63, input_ch_views=27, skips=[2], use_viewdirs=True,
                             precision='int8')
     render_kwargs_train, ... = create_nerf(args)        # args.precision = 'int8'

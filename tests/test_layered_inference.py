@@ -178,3 +178,64 @@ def test_a_concatenated_layer_adds_its_parts_in_32_bits(gpu, W):
         want = want + dequantised(rows) @ (p * s)
         mag = mag + (dequantised(rows) @ (p * s)).abs()
     close(run.raw[:, 3:], want, 5.001 * 2.0 ** -24 * mag, "alpha")
+
+
+def _float_network(net, pe, ve):
+    """(raw, variance) of the network on 64-bit parameters and encodings, and the variance of raw that its 8-bit layers'
+    roundings give if they are independent: a step s has s^2 / 12, for the rows (the next power of two of their largest
+    value over 127) and for the channels of W."""
+    def step2(x, dim):
+        top = x.abs().amax(dim, keepdim=True)
+        return torch.exp2(torch.ceil(torch.log2((top / 127).clamp_min(2.0 ** -126)))) ** 2 / 12
+
+    def layer(i, parts):
+        z, var = net.bias(i).detach().double().to(pe.device), 0
+        for (x, vx), (r0, k, _) in zip(parts, net.split(i)):
+            w = net.weight(i)[r0:r0 + k].detach().double().to(pe.device)
+            vw = step2(w, 0).expand_as(w)
+            z = z + x @ w
+            var = var + vx @ (w * w + vw) + (x * x) @ vw
+        return z, var
+
+    def rows(z, var):
+        return z, var + step2(z, 1)
+
+    def relu(z, var):
+        return z.clamp(min=0), var * (z > 0)
+    e, v = rows(pe, torch.zeros_like(pe)), rows(ve, torch.zeros_like(ve))
+    h = [e]
+    for i in range(net.D):
+        y = rows(*relu(*layer(i, h)))
+        h = [e, y] if i in net.skips else [y]
+    a, va = layer(net.D + 3, h)
+    y = rows(*relu(*layer(net.D + 1, [rows(*layer(net.D, h)), v])))
+    c, vc = layer(net.D + 2, [y])
+    return torch.cat([c, a], 1), torch.cat([vc, va], 1)
+
+
+def _points(n, far, seed, device):
+    g = torch.Generator().manual_seed(seed)
+    pts = (torch.rand((n, 3), generator=g) * 2 - 1) * far
+    vd = torch.nn.functional.normalize(torch.randn((n, 3), generator=g), dim=1)
+    return pts.to(device), vd.to(device)
+
+
+def _encoded(x, channels):
+    x = x.double()
+    return torch.cat([x] + [f(x * 2.0 ** i) for i in range((channels - 3) // 6) for f in (torch.sin, torch.cos)], 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("far", [0.5, 2.0, 6.0])
+@pytest.mark.parametrize("change", [dict(D=8, W=256, input_ch=63, input_ch_views=27, skips=[4]), dict(D=4, W=128, skips=[0, 3]), dict(D=3, W=640)])
+def test_the_network_as_a_whole_is_off_by_its_roundings(gpu, change, far):
+    """Against the same network in 64 bits: what 8-bit rows and weights of the stated steps give, taken as independent;
+    twice that, for what they have in common (a row's or a channel's errors share a scale, points share the weights)."""
+    from nerf_amd import layered
+    from nerf_amd.run_nerf_helpers import init_nerf_model
+    net = init_nerf_model(**{**SHAPE, **change}, device=gpu, generator=torch.Generator(device=gpu).manual_seed(11), precision='int8')
+    pts, vd = _points(3000, far, 12, gpu)
+    want, var = _float_network(net, _encoded(pts, net.input_ch), _encoded(vd, net.input_ch_views))
+    err = layered.query(net, pts, vd, 1).double() - want
+    rms, expected = err.pow(2).mean(0).sqrt(), var.mean(0).sqrt()
+    assert bool((rms <= 2 * expected).all()), (rms / expected).tolist()
