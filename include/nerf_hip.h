@@ -299,8 +299,8 @@ int nerf_adam_step(float* theta, const float* g, float* m, float* v, int64_t n, 
  *
  * Rows in 8 bits: q [n][kp], kp = k rounded up to 64, zeros behind column k; scale [n].  An element is
  * q * scale.  scale = max|x| / 127 of the row (0, and zeros, below 2^-100), or with pow2 the smallest
- * power of two at or above that, at least 2^-126; q = x / scale rounded, halves to even.  A row that
- * holds an infinity or NaN gets the scale NaN and zeros.
+ * power of two at or above that, at least 2^-126; q = x times the inverse (127 / max|x|, or 1 / scale),
+ * rounded, halves to even.  A row that holds an infinity or NaN gets the scale NaN and zeros.
  * mask: [n][kp / 8] bytes or NULL; bit f & 7 of byte f >> 3 = (x[f] > 0): what the gradient of a ReLU
  * whose output x is needs.  q must be 16-byte aligned. */
 int nerf_quantize_rows(const void* x, int dtype, int64_t n, int k, int64_t ldx, int pow2, signed char* q,
@@ -321,8 +321,8 @@ int nerf_linear_int8(const signed char* q, const float* scale, int64_t n, int k,
                      const float* bias, const void* addend, int addend_dtype, int64_t ldadd, int relu,
                      void* y, int dtype, int64_t ldy, nerf_stream_t stream);
 
-/* nerf_quantize_rows of that y (in fp32, never stored): the next layer's rows, yq [n][m rounded up to 64].
- * With an addend m must be a multiple of 64, otherwise NERF_E_UNSUPPORTED.  workspace:
+/* nerf_quantize_rows of that y (in fp32, never stored): the next layer's rows, yq [n][m rounded up to 64],
+ * which must not overlap an input.  With an addend m must be a multiple of 64, otherwise NERF_E_UNSUPPORTED.  workspace:
  * nerf_linear_int8_quantized_bytes(n, m) bytes (0 up to 512 outputs: NULL will do). */
 size_t nerf_linear_int8_quantized_bytes(int64_t n, int m);
 int nerf_linear_int8_quantized(const signed char* q, const float* scale, int64_t n, int k, const void* packed, int m,
@@ -332,7 +332,9 @@ int nerf_linear_int8_quantized(const signed char* q, const float* scale, int64_t
 
 /* dx [n][k] = dz [n][m] times the transposed weights as the forward pass used them (packed with pow2 only:
  * they are then exact in bf16), zero where the bit of `mask` is 0.  dz is taken as the exact sum of 1, 2
- * or 3 bf16 terms (bf16, fp16, fp32): every product is exact, sums are fp32.  dx has dz's type. */
+ * or 3 bf16 terms (bf16, fp16, fp32; a term below 2^-126 may be lost): every product is exact, sums are fp32;
+ * infinities and NaN go through the products as they do in the formula.  dx has dz's type and must not
+ * overlap an input. */
 int nerf_linear_int8_grad_input(const void* dz, int dtype, int64_t n, int m, int64_t lddz, const void* packed, int k,
                                 const unsigned char* mask, void* dx, int64_t lddx, nerf_stream_t stream);
 
