@@ -4,6 +4,7 @@ Same names, argument meaning and return structure as the reference (file:line ci
 function), so `from nerf_amd.run_nerf_helpers import *` can replace the reference's star import
 (run_nerf.py:7).  All arithmetic runs in libnerfhip.so on the GPU.
 """
+import threading
 import weakref
 
 import numpy as np
@@ -90,6 +91,7 @@ class LaidOut:
         self.device, self.memory, self.version = device, None, None
         self.stream = self.event = None   # where the last layout was queued, and the point behind it
         self.known = set()                # streams the allocator knows to use the memory
+        self.lock = threading.Lock()
 
     def __reduce__(self):                 # a copy of a network lays out its own
         return LaidOut, (self.device,)
@@ -103,7 +105,7 @@ class LaidOut:
         stream = torch._C._cuda_getCurrentRawStream(self.device.index)
         if version == self.version and stream == self.stream:
             return self.memory
-        with torch.no_grad(), torch.cuda.device(self.device):
+        with self.lock, torch.no_grad(), torch.cuda.device(self.device):
             capturing = torch.cuda.is_current_stream_capturing()   # (a capture begins with the device idle)
             here = torch.cuda.current_stream()
             if not capturing and self.event is not None and stream != self.stream:
@@ -111,13 +113,15 @@ class LaidOut:
             if version != self.version:
                 self.memory = lay(self.memory)
                 if not capturing:
-                    self.version, self.stream, self.event = version, stream, torch.cuda.Event()
-                    self.event.record(here)
+                    event = torch.cuda.Event()
+                    event.record(here)
+                    self.stream, self.event = stream, event
+                    self.version = version                          # last: another thread may look without the lock
             if not capturing and stream not in self.known:
                 self.known.add(stream)
                 for t in tensors(self.memory):
                     t.record_stream(here)
-        return self.memory
+            return self.memory
 
 
 class NerfModel:

@@ -124,6 +124,34 @@ def test_two_streams_query_one_network_that_has_just_changed(gpu, precision):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("precision", ['int8', None])
+def test_two_host_threads_query_one_network_that_has_just_changed(gpu, precision):
+    import threading
+    (net, other), query = _networks(gpu, precision)
+    rays, z = _rays(gpu, 40, 6)
+    want = [query(m, rays, z) for m in (net, other)]
+    weights = [[w.copy() for w in m.get_weights()] for m in (net, other)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for turn in range(8):
+        net.set_weights(weights[(turn + 1) % 2])
+        torch.cuda.synchronize()
+        start, got = threading.Barrier(2), [None, None]
+
+        def work(i):
+            torch.cuda.set_device(gpu)
+            with torch.cuda.stream(streams[i]):
+                start.wait()
+                got[i] = query(net, rays, z)
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, want[(turn + 1) % 2]) for a in got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("precision", ['int8', None])
 def test_a_copied_network_lays_out_its_own_weights(gpu, precision):
     import copy
     (net, other), query = _networks(gpu, precision)
