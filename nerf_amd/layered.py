@@ -27,7 +27,7 @@ from . import ops
 from .run_nerf_helpers import LaidOut, NerfModel
 
 # Points evaluated at a time when nothing is recorded: no more than these, and as many as the network's widest layer
-# leaves within these bytes of transient memory (one 256 wide takes 2.3 GiB for its 2^20, one 4096 wide 89 thousand points).
+# leaves within these bytes of transient memory (256 wide: at most 3.1 GiB for 2^20; 4096 wide: 103 thousand points).
 _QUERY_POINTS = 1 << 20
 _QUERY_BYTES = 4 << 30
 

@@ -491,6 +491,7 @@ class GraphedTrainStep:
     The optimiser step runs outside the graph (its learning rate changes every step and is a
     kernel argument).  The automatic fp16 gradient scale keeps looking after itself: the status
     blocks are read between replays, and the step is captured anew when a network's target moved.
+    Hooks registered on the parameters are captured with the step (those of that moment).
     Single process only (no gradient exchange inside the graph)."""
 
     def __init__(self, render_fn, n_rays, grad_vars, optimizer, models, device=None):

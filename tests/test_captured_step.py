@@ -63,3 +63,33 @@ def test_hooks_of_parameters_take_part_in_a_capture():
     want = [torch.full_like(p, i + 1.) for i, p in enumerate(net.params)]
     want[0] = want[0] * 3 + 1
     assert all(torch.equal(a, b) for a, b in zip(out[0], want)) and calls == [3. * net.params[2].numel()]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("precision", ['int8', None])
+def test_one_network_for_both_passes_captured(gpu, precision):
+    """... listed once and twice, with a hook that halves a gradient: the bits of train_step."""
+    from nerf_amd import training
+    from nerf_amd.run_nerf import create_nerf, render
+    from tests.util import default_args
+    runs = []
+    for listed in (0, 1, 2):
+        torch.manual_seed(8)
+        a = default_args()
+        a.precision, a.N_samples, a.N_importance, a.no_reload = precision, 12, 9, True
+        kw = {**create_nerf(a)[0], 'perturb': 0., 'network_fine': None}
+        net = kw['network_fn']
+        opt = training.Adam(5e-4).bind_models([net])
+        net.params[2].register_hook(lambda g: g * 0.5)
+        fn = lambda r: render(8, 8, 9.0, chunk=1024, rays=r, near=2., far=6., retraw=True, **kw)
+        g = torch.Generator(device=gpu).manual_seed(9)
+        step = training.GraphedTrainStep(fn, 32, net.params, opt, [net] * listed) if listed else None
+        log = []
+        for _ in range(4):
+            o = torch.nn.functional.normalize(torch.randn((32, 3), generator=g, device=gpu), dim=1) * 4
+            t = torch.rand((32, 3), generator=g, device=gpu)
+            loss = (step((o, -o / 4), t) if listed else training.train_step(fn, (o, -o / 4), t, net.params, opt))[0]
+            log.append(loss.detach().clone())
+            assert bool(torch.isfinite(fn((o, -o / 4))[0]).all())    # eager work between the replays
+        runs.append([torch.stack(log), net.flat.detach().clone()])
+    assert all(torch.equal(x, y) for r in runs[1:] for x, y in zip(r, runs[0]))
